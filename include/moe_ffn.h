@@ -61,7 +61,10 @@ enum {
 enum {
     MOE_DEVFLAG_BAD_ID = 1,   /* an expert id > n_experts was seen; its slot was dropped */
     MOE_DEVFLAG_DUP_ID = 2,   /* a token named one expert in two slots; the later was dropped */
-    MOE_DEVFLAG_TIMEOUT = 4   /* moe_decode_stack: a bounded wait expired; its output is invalid */
+    MOE_DEVFLAG_TIMEOUT = 4,  /* moe_decode_stack: a bounded wait expired; its output is invalid */
+    MOE_DEVFLAG_BAD_PAGE = 8, /* attention: a page id outside the cache; its tokens were left out */
+    MOE_DEVFLAG_BAD_SEQ = 16  /* attention: a sequence's length or rows out of range; what lies
+                                 outside was left out */
 };
 
 typedef struct {
@@ -253,6 +256,100 @@ moe_status moe_stack_spin_limit(moe_ctx *ctx, uint32_t polls);
  * numbering is k_stack.hip's StackTraceEvent).  buf = NULL stops it.  Other builds return
  * MOE_EUNSUPPORTED. */
 moe_status moe_stack_trace(moe_ctx *ctx, uint64_t *buf, size_t words);
+
+/* ---- attention over a paged key-value cache ----
+ * What a layer of the same model computes between two MoE calls: the new tokens' keys and
+ * values are written into the cache (moe_kv_append), then every new token attends to its
+ * sequence's cached tokens up to its own (moe_attn_decode: one new token of each sequence;
+ * moe_attn_prompt: any number).  Replaces the KvWrite and Attention dispatches of
+ * record_and_submit_layer (src/inference.rs:529-545: shaders/kv_write.comp, attention.comp).
+ *
+ * A moe_attn holds one layer shape and its workspaces, as a moe_ctx does: one stream/thread
+ * at a time (graphs captured from one moe_attn share its workspaces: replay them in order on
+ * one stream, or capture them from handles of their own), no allocation after creation.  A
+ * call runs on the handle's device whatever the current one is; `stream` belongs to it. */
+typedef struct moe_attn moe_attn;
+
+/* Element types, by their GGML type ids. */
+enum { MOE_T_F32 = 0, MOE_T_F16 = 1, MOE_T_BF16 = 30 };
+
+typedef struct {
+    int n_q_heads;   /* 1..256, a multiple of n_kv_heads: query head h reads key-value head
+                        h / (n_q_heads / n_kv_heads) */
+    int n_kv_heads;
+    int head_dim;    /* 64, 128 or 256 */
+    int page_tokens; /* tokens of a cache page: a power of two, 16..1024 */
+    int type;        /* of the cache, the queries and the outputs: MOE_T_F16 or MOE_T_BF16 */
+    int max_seqs;    /* most sequences of a call, 1..65535 */
+} moe_attn_config;
+
+/* A cache: element (page, head, token, i) of the keys at
+ *   k + page * page_stride + head * head_stride + token * token_stride + i   (elements),
+ * the values with the same strides from v.  Any order of page, head and token; strides are
+ * positive multiples of 8 elements, k and v 16-byte aligned, i contiguous. */
+typedef struct {
+    void *k, *v;
+    int n_pages;
+    int64_t page_stride, head_stride, token_stride;
+} moe_kv_cache;
+
+/* The sequences of a call, in device memory that the call reads when it runs: of sequence b
+ * the cached tokens' pages pages[b * pages_stride + 0..max_pages-1] (place t in page t /
+ * page_tokens; entries behind the last used page are not read), the number of cached tokens
+ * kv_len[b], the new ones included, and its rows row_start[b]..row_start[b+1]-1 of the packed
+ * row arrays (row_start ascends; the last row is the last new token).  row_start = NULL: one
+ * row a sequence.  n_rows: rows of the packed arrays; those of no sequence (behind the last
+ * one's, say) are left as they were. */
+typedef struct {
+    int n_seqs;
+    int n_rows;
+    const int32_t *pages;
+    int64_t pages_stride;
+    int max_pages;
+    const int32_t *kv_len;
+    const int32_t *row_start;
+} moe_seq_batch;
+
+/* Checks the shape and allocates every workspace (nothing is allocated later).  MOE_EUNSUPPORTED:
+ * a head_dim or type that is not compiled. */
+moe_status moe_attn_create(int device, const moe_attn_config *cfg, moe_attn **out);
+moe_status moe_attn_destroy(moe_attn *a);
+
+/* Write the new tokens' keys and values, k and v [n_rows][n_kv_heads][head_dim] with rows
+ * k_row_stride / v_row_stride elements apart (a slice of a fused projection's rows: multiples of 16
+ * bytes; 16-byte aligned), to the places kv_len[b] - n_b .. kv_len[b] - 1 of their sequences.
+ * in_type: the cache's type, or MOE_T_F32 (rounded to nearest even).  Tokens whose place is
+ * negative, behind the page list or in a page outside the cache are left out and flagged.  Two
+ * tokens with the same place (a page that two sequences share): either one's row ends there. */
+moe_status moe_kv_append(moe_attn *a, const moe_kv_cache *kv, const moe_seq_batch *seqs, const void *k,
+                         const void *v, int in_type, int64_t k_row_stride, int64_t v_row_stride, void *stream);
+
+/* One new token of every sequence over its cached tokens 0..kv_len[b]-1 (row_start must be NULL):
+ *   o[b][h] = sum_j softmax_j(scale * q[b][h] . K_j) V_j,   lse[b][h] = log(sum_j exp(scale * q[b][h] . K_j))
+ * q, o: rows of n_q_heads heads, q_row_stride / o_row_stride elements apart (multiples of 8,
+ * 16-byte aligned), head_dim contiguous.  lse f32 [n_rows][n_q_heads] or NULL.  Scores, maxima,
+ * sums and products are held in f32.  A row that sees no token (kv_len 0) gets o = 0 and lse =
+ * -inf.  Tokens not cached (behind kv_len) are never used, whatever their places hold.  A length
+ * below 0 or behind the page list is taken as the nearest in range, and the tokens of a page
+ * outside the cache are left out; both are flagged (moe_attn_flags).  o may be q itself
+ * (same address and stride); otherwise outputs overlap no input. */
+moe_status moe_attn_decode(moe_attn *a, const moe_kv_cache *kv, const moe_seq_batch *seqs, const void *q,
+                           int64_t q_row_stride, float scale, void *o, int64_t o_row_stride, float *lse,
+                           void *stream);
+
+/* The same for packed prompts or pieces of them: row i of sequence b (n_b rows) sees the tokens
+ * 0 .. kv_len[b] - n_b + i, so a prompt, and a prompt's next piece over what is cached already.
+ * Rows in front of the cache (kv_len[b] < n_b) see nothing.  A token that a row does not see does
+ * not reach its output, whatever it holds (infinities and NaN too). */
+moe_status moe_attn_prompt(moe_attn *a, const moe_kv_cache *kv, const moe_seq_batch *seqs, const void *q,
+                           int64_t q_row_stride, float scale, void *o, int64_t o_row_stride, float *lse,
+                           void *stream);
+
+/* Synchronise `stream` and return (then clear) the handle's sticky flags MOE_DEVFLAG_BAD_PAGE and
+ * MOE_DEVFLAG_BAD_SEQ. */
+moe_status moe_attn_flags(moe_attn *a, void *stream, uint32_t *flags);
+/* moe_device_flags_async for a moe_attn: one tiny launch moves the flags into *dst. */
+moe_status moe_attn_flags_async(moe_attn *a, uint32_t *dst, void *stream);
 
 /* Last error message of the calling thread ("" when none). */
 const char *moe_last_error(void);

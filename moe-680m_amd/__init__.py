@@ -13,6 +13,8 @@ Reference interfaces mirrored (path:line in the reference tree):
                               the GPU top-k read back by do_route (src/inference.rs:622-659)
   ``Context.bucket_fill``  -- router::build_expert_batches (src/router.rs:55-97)
   ``Context.ffn``          -- InferenceEngine::record_and_submit_moe (src/inference.rs:663-766)
+  ``AttnContext``          -- the KvWrite and Attention dispatches of record_and_submit_layer
+                              (src/inference.rs:529-545)
   ``Context.ffn_route``    -- the RouterTopk dispatch + do_route + record_and_submit_moe of one
                               layer (src/inference.rs:608-616, 622-766)
 """
@@ -40,8 +42,11 @@ W_REF, W_RENORM = 0, 1
 COPIES_AUTO, COPIES_SPLIT, COPIES_BOTH = 0, 1, 2
 FFN_ACCUMULATE, FFN_RMSNORM, STACK_ROUTE_GEMV = 1, 2, 4
 DEVFLAG_BAD_ID, DEVFLAG_DUP_ID, DEVFLAG_TIMEOUT = 1, 2, 4
+DEVFLAG_BAD_PAGE, DEVFLAG_BAD_SEQ = 8, 16
 # Router gate matrix element types (GGML type ids, include/moe_ffn.h MOE_WG_*).
 WG_F32, WG_F16, WG_IQ4_XS = 0, 1, 23
+# Element types of the attention calls (GGML type ids, include/moe_ffn.h MOE_T_*).
+T_F32, T_F16, T_BF16 = 0, 1, 30
 
 # Every symbol include/moe_ffn.h declares (checked by the CPU test suite).
 EXPORTS = (
@@ -50,6 +55,8 @@ EXPORTS = (
     "moe_ffn", "moe_ffn_route", "moe_ffn_noalloc", "moe_decode_stack", "moe_dequant_iq4xs", "moe_device_flags",
     "moe_device_flags_async", "moe_stack_spin_limit", "moe_stack_trace", "moe_last_error",
     "moe_timing_enable", "moe_timing_read",
+    "moe_attn_create", "moe_attn_destroy", "moe_kv_append", "moe_attn_decode", "moe_attn_prompt", "moe_attn_flags",
+    "moe_attn_flags_async",
     "moe_gen_iq4xs", "moe_gen_normal", "moe_gen_logits",
 )
 
@@ -75,6 +82,22 @@ class _LayerWeights(ctypes.Structure):
                 ("shared_w3", ctypes.c_void_p), ("shared_w2", ctypes.c_void_p)]
 
 
+class _AttnConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("n_q_heads", "n_kv_heads", "head_dim", "page_tokens", "type", "max_seqs")]
+
+
+class _KVCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("n_pages", ctypes.c_int),
+                ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("token_stride", ctypes.c_int64)]
+
+
+class _SeqBatch(ctypes.Structure):
+    _fields_ = [("n_seqs", ctypes.c_int), ("n_rows", ctypes.c_int), ("pages", ctypes.c_void_p),
+                ("pages_stride", ctypes.c_int64), ("max_pages", ctypes.c_int), ("kv_len", ctypes.c_void_p),
+                ("row_start", ctypes.c_void_p)]
+
+
 _lib = None
 
 
@@ -88,6 +111,7 @@ def lib():
                           "(make -C moe-680m_amd); there is no fallback path")
     L = ctypes.CDLL(LIB_PATH)
     vp, i, u64, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_size_t
+    i64 = ctypes.c_int64
     sigs = {
         "moe_create": [i, ctypes.POINTER(_Config), ctypes.POINTER(vp)],
         "moe_create_with": [i, ctypes.POINTER(_Config), i, ctypes.POINTER(vp)],
@@ -111,6 +135,13 @@ def lib():
         "moe_gen_iq4xs": [vp, sz, u64, u64, vp],
         "moe_gen_normal": [vp, sz, u64, u64, ctypes.c_float, ctypes.c_float, vp],
         "moe_gen_logits": [vp, i, i, u64, i, ctypes.c_double, ctypes.c_double, vp],
+        "moe_attn_create": [i, ctypes.POINTER(_AttnConfig), ctypes.POINTER(vp)],
+        "moe_attn_destroy": [vp],
+        "moe_kv_append": [vp, vp, vp, vp, vp, i, i64, i64, vp],
+        "moe_attn_decode": [vp, vp, vp, vp, i64, ctypes.c_float, vp, i64, vp, vp],
+        "moe_attn_prompt": [vp, vp, vp, vp, i64, ctypes.c_float, vp, i64, vp, vp],
+        "moe_attn_flags": [vp, vp, ctypes.POINTER(ctypes.c_uint32)],
+        "moe_attn_flags_async": [vp, vp, vp],
         "moe_timing_enable": [vp, i],
         "moe_timing_read": [vp, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(ctypes.c_double)],
     }
@@ -363,6 +394,168 @@ class Context:
         ms = (ctypes.c_double * n)()
         _check(lib().moe_timing_read(self._h, counts, ms))
         return {k: (counts[i], ms[i]) for i, k in enumerate(KERNELS) if counts[i]}
+
+
+_ATTN_TYPES = {torch.float16: T_F16, torch.bfloat16: T_BF16, torch.float32: T_F32}
+
+
+class KVCache:
+    """One layer's paged key-value cache: k, v device tensors [n_pages][n_kv_heads][page_tokens]
+    [head_dim] of float16 or bfloat16, both with the same strides; a view in another order (a
+    [n_pages][page_tokens][n_kv_heads][head_dim] tensor's transpose(1, 2)) will do.  Made once and
+    kept: it holds the tensors."""
+
+    def __init__(self, k, v):
+        if k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride():
+            raise ValueError("k and v: [n_pages][n_kv_heads][page_tokens][head_dim], the same strides")
+        if k.dtype != v.dtype or k.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"cache dtypes {k.dtype} and {v.dtype}: float16 or bfloat16, the same")
+        if k.device != v.device:
+            raise ValueError("k and v lie on different devices")
+        if k.stride(3) != 1:
+            raise ValueError("the last dimension of a cache must be contiguous")
+        self.k, self.v, self.dtype, self.device = k, v, k.dtype, k.device
+        self.shape = tuple(k.shape[1:])  # heads, page tokens, head_dim
+        # a dimension of one has no stride of its own
+        st = [k.stride(i) if k.shape[i] > 1 else k.shape[3] for i in range(3)]
+        self._c = _KVCache(k.data_ptr(), v.data_ptr(), k.shape[0], *st)
+        self._ref = ctypes.addressof(self._c)
+
+
+class SeqBatch:
+    """The sequences of attention calls (moe_seq_batch): pages int32 [n_seqs][max_pages], kv_len
+    int32 [n_seqs] (cached tokens, the new ones included), row_start int32 [n_seqs + 1] for packed
+    rows (None: one row a sequence), n_rows the rows of the packed arrays.  Made once and kept
+    for all layers of a step, or longer: the calls read the tensors' contents when they run."""
+
+    def __init__(self, pages, kv_len, row_start=None, n_rows=None):
+        for name, t, dim in (("pages", pages, 2), ("kv_len", kv_len, 1), ("row_start", row_start, 1)):
+            if t is None:
+                continue
+            if t.dtype != torch.int32 or t.dim() != dim or t.device != pages.device:
+                raise ValueError(f"{name}: an int32 tensor of {dim} dimension(s), all on one device")
+            if t.shape[-1] > 1 and t.stride(-1) != 1:
+                raise ValueError(f"{name} must be contiguous")
+        n = pages.shape[0]
+        if kv_len.shape[0] != n or (row_start is not None and row_start.shape[0] != n + 1):
+            raise ValueError("kv_len holds a length, row_start one more start, for each row of pages")
+        if n_rows is None:
+            if row_start is not None:
+                raise ValueError("n_rows is required with row_start")
+            n_rows = n
+        if row_start is None and n_rows != n:
+            raise ValueError("one row a sequence without row_start")
+        self.pages, self.kv_len, self.row_start, self.n_rows = pages, kv_len, row_start, n_rows
+        self.device = pages.device
+        stride = pages.stride(0) if n > 1 else pages.shape[1]
+        self._c = _SeqBatch(n, n_rows, pages.data_ptr(), stride, pages.shape[1], kv_len.data_ptr(),
+                            None if row_start is None else row_start.data_ptr())
+        self._ref = ctypes.addressof(self._c)
+
+
+class AttnContext:
+    """One moe_attn: the shape of an attention layer and its workspaces (include/moe_ffn.h).  One
+    stream at a time; the layers of a model share one."""
+
+    def __init__(self, n_q_heads, n_kv_heads, head_dim, page_tokens, max_seqs, dtype=torch.float16, device=0):
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"dtype {dtype}: float16 or bfloat16")
+        self.n_q_heads, self.n_kv_heads, self.head_dim = n_q_heads, n_kv_heads, head_dim
+        self.page_tokens, self.max_seqs, self.dtype = page_tokens, max_seqs, dtype
+        self.device = torch.device("cuda", device)
+        self._h = None
+        cfg = _AttnConfig(n_q_heads, n_kv_heads, head_dim, page_tokens, _ATTN_TYPES[dtype], max_seqs)
+        h = ctypes.c_void_p()
+        _check(lib().moe_attn_create(device, ctypes.byref(cfg), ctypes.byref(h)))
+        self._h = h
+        self._shape = (n_kv_heads, page_tokens, head_dim)
+        self._decode, self._prompt = lib().moe_attn_decode, lib().moe_attn_prompt
+
+    @property
+    def handle(self):
+        return self._h
+
+    def close(self):
+        if self._h is not None and self._h.value:
+            _check(lib().moe_attn_destroy(self._h))
+        self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _checked(self, cache, batch):
+        if self._h is None:
+            raise ValueError("the context is closed")
+        if cache.shape != self._shape or cache.dtype != self.dtype:
+            raise ValueError(f"a cache of {cache.shape} {cache.dtype}, not {self._shape} {self.dtype}")
+        if cache.device != self.device or batch.device != self.device:
+            raise ValueError(f"cache on {cache.device}, sequences on {batch.device}: the context is on {self.device}")
+
+    def _rows(self, name, t, batch, heads):
+        if t.shape != (batch.n_rows, heads, self.head_dim):
+            raise ValueError(f"{name} of {tuple(t.shape)}, not {(batch.n_rows, heads, self.head_dim)}")
+        if t.device != self.device:
+            raise ValueError(f"{name} on {t.device}: the context is on {self.device}")
+        row, head, one = t.stride()
+        if one != 1 or (heads > 1 and head != self.head_dim):
+            raise ValueError(f"{name}: a row's heads must be contiguous")
+        return row if batch.n_rows > 1 else heads * self.head_dim
+
+    def _on(self, stream):
+        return torch.cuda.current_stream(self.device).cuda_stream if stream is None else _stream(stream)
+
+    def kv_append(self, cache, batch, k, v, stream=None):
+        """Write the packed rows k, v [n_rows][n_kv_heads][head_dim] (the cache's dtype or float32;
+        a slice of a fused projection's rows will do) to their sequences' last places."""
+        self._checked(cache, batch)
+        if k.dtype != v.dtype or k.dtype not in (self.dtype, torch.float32):
+            raise ValueError(f"rows of {k.dtype} and {v.dtype}: {self.dtype} or float32, the same")
+        ks, vs = self._rows("k", k, batch, self.n_kv_heads), self._rows("v", v, batch, self.n_kv_heads)
+        _check(lib().moe_kv_append(self._h, cache._ref, batch._ref, k.data_ptr(), v.data_ptr(), _ATTN_TYPES[k.dtype],
+                                   ks, vs, self._on(stream)))
+
+    def _attend(self, call, cache, batch, q, scale, o, lse, stream):
+        self._checked(cache, batch)
+        qs = self._rows("q", q, batch, self.n_q_heads)
+        if o is None:
+            o = torch.empty((batch.n_rows, self.n_q_heads, self.head_dim), dtype=self.dtype, device=self.device)
+            os_ = self.n_q_heads * self.head_dim
+        else:
+            os_ = self._rows("o", o, batch, self.n_q_heads)
+        if q.dtype != self.dtype or o.dtype != self.dtype:
+            raise ValueError(f"q of {q.dtype}, o of {o.dtype}: the context's dtype is {self.dtype}")
+        if lse is not None and (lse.dtype != torch.float32 or lse.shape != (batch.n_rows, self.n_q_heads)
+                                or not lse.is_contiguous() or lse.device != self.device):
+            raise ValueError("lse: a contiguous float32 tensor [n_rows][n_q_heads] on the context's device")
+        _check(call(self._h, cache._ref, batch._ref, q.data_ptr(), qs, self.head_dim ** -0.5 if scale is None else scale,
+                    o.data_ptr(), os_, _ptr(lse), self._on(stream)))
+        return o
+
+    def attn_decode(self, cache, batch, q, scale=None, o=None, lse=None, stream=None):
+        """One new token of every sequence over its cached tokens (moe_attn_decode): q [n_seqs]
+        [n_q_heads][head_dim], scale 1/sqrt(head_dim) unless given; returns o, of q's shape."""
+        return self._attend(self._decode, cache, batch, q, scale, o, lse, stream)
+
+    def attn_prompt(self, cache, batch, q, scale=None, o=None, lse=None, stream=None):
+        """Packed prompts, or pieces of them, causal over the cache that holds their keys and values
+        already (moe_attn_prompt): q [n_rows][n_q_heads][head_dim]; returns o, of q's shape, in
+        which rows of no sequence are left as they were."""
+        return self._attend(self._prompt, cache, batch, q, scale, o, lse, stream)
+
+    def device_flags(self, stream=None):
+        """Synchronise, return and clear the sticky flags (DEVFLAG_BAD_PAGE, DEVFLAG_BAD_SEQ)."""
+        v = ctypes.c_uint32()
+        _check(lib().moe_attn_flags(self._h, self._on(stream), ctypes.byref(v)))
+        return v.value
+
+    def device_flags_async(self, dst, stream=None):
+        """Enqueue the move of the sticky flags into dst (a 1-element int32/uint32 tensor on the
+        device or in pinned host memory)."""
+        _check(lib().moe_attn_flags_async(self._h, _ptr(dst), self._on(stream)))
+        return dst
 
 
 def dequant_iq4xs(blocks, out=None, stream=None):

@@ -1,0 +1,40 @@
+// attn_internal.hpp -- argument block and launchers of the attention kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "moe_ffn.h"
+
+namespace moe {
+
+// One call's sequences, cache and rows (see moe_seq_batch and moe_kv_cache for the layout).
+struct AttnArgs {
+    const void *q;
+    void *o;
+    float *lse;               // or null
+    int64_t q_stride, o_stride; // elements between rows
+    uint8_t *k, *v;
+    int64_t page_stride, head_stride, token_stride; // elements
+    const int32_t *pages;
+    int64_t pages_stride;
+    const int32_t *kv_len, *row_start;
+    uint32_t *flags;
+    int n_pages, max_pages, page_shift;
+    int n_seqs, n_rows;
+    int hq, hkv, group;       // group = hq / hkv
+    float scale_log2;         // scale * log2(e): exponentials are taken in base 2
+};
+
+struct AppendArgs {
+    const uint8_t *src[2];    // new keys, new values
+    uint8_t *dst[2];
+    int64_t src_stride[2];    // bytes between rows
+    AttnArgs c;
+};
+
+hipError_t launch_kv_append(const AppendArgs &a, int type, int in_type, int d, hipStream_t st);
+hipError_t launch_attn(const AttnArgs &a, int type, int d, hipStream_t st);
+hipError_t launch_attn_flags(uint32_t *flags, uint32_t *dst, hipStream_t st);
+
+} // namespace moe

@@ -1,0 +1,598 @@
+"""GPU: the paged key-value cache's write and the attention over it (decode and prompt) against a
+plain 64-bit implementation, element by element within bounds derived in attn_util."""
+import math
+
+import pytest
+
+from attn_util import Setup, TYPES, check
+from gpu_util import log
+
+pytestmark = pytest.mark.gpu
+
+MODEL = (16, 2, 256)
+
+
+def run_decode(gpu, s, ref=True, **kw):
+    import torch
+    ctx = s.context(gpu)
+    k, v = s.pools()
+    q = s.q.cuda()
+    lse = torch.full((s.n_rows, s.hq), 77.0, device="cuda")
+    call = ctx.attn_decode if s.rows is None else ctx.attn_prompt
+    o = torch.full((s.n_rows, s.hq, s.d), 55.0, dtype=s.type, device="cuda")
+    call(gpu.KVCache(k, v), s.seqs(gpu), q, o=o, lse=lse, **kw)
+    flags = ctx.device_flags()
+    if not ref:
+        return o, lse, flags
+    want, bound, wl, lb = s.reference(kw.get("scale"))
+    rows = [r for r, _, _ in s.row_seen()]
+    rest = [r for r in range(s.n_rows) if r not in set(rows)]
+    check("o", o[rows], want[rows], bound[rows])
+    seen = [r for r, _, n in s.row_seen() if n]
+    check("lse", lse[seen], wl[seen], lb[seen])
+    for r in set(rows) - set(seen):
+        assert (lse[r] == -math.inf).all()
+    assert (o[rest] == 55.0).all() and (lse[rest] == 77.0).all()
+    assert flags == 0
+    return o, lse, flags
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("heads", [MODEL, (32, 8, 128), (12, 12, 64), (8, 1, 128), (24, 1, 64), (40, 2, 128), (3, 1, 256),
+                                   (17, 1, 64)])
+def test_decode_heads_and_lengths(gpu, heads, type):
+    log(f"decode heads {heads} {type}")
+    run_decode(gpu, Setup(*heads, 16, type, [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 300, 1000],
+                          seed=1))
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 512, 1024])
+@pytest.mark.parametrize("order", ["hnd", "nhd", "mixed"])
+def test_decode_pages_and_orders(gpu, page, order):
+    log(f"decode page {page} {order}")
+    run_decode(gpu, Setup(*MODEL, page, "bf16", [257, 0, 1025, 90], order=order, seed=2))
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_decode_long_single_sequences(gpu, type):
+    """Split over the length: one or two sequences of many pages."""
+    log(f"decode long {type}")
+    run_decode(gpu, Setup(4, 2, 64, 16, type, [20011], seed=3))
+    run_decode(gpu, Setup(4, 1, 128, 64, type, [9001, 5], seed=4))
+
+
+def test_decode_many_sequences(gpu):
+    log("decode 1500 sequences")
+    kv = [(37 * b) % 53 for b in range(1500)]
+    run_decode(gpu, Setup(2, 1, 64, 16, "f16", kv, seed=5))
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("heads", [MODEL, (32, 8, 128), (12, 12, 64), (24, 1, 64), (40, 2, 128), (3, 1, 256), (200, 1, 64)])
+def test_prompt_heads_and_rows(gpu, heads, type):
+    """Packed sequences of 0, 1 and odd numbers of rows, with and without cached tokens before them,
+    and rows in front of the cache."""
+    log(f"prompt heads {heads} {type}")
+    rows = [1, 0, 5, 17, 64, 33, 3, 2, 70]
+    before = [0, 40, 0, 100, 0, 1, -2, -2, 300]
+    run_decode(gpu, Setup(*heads, 16, type, [r + c for r, c in zip(rows, before)], rows, seed=6, extra_rows=3))
+
+
+@pytest.mark.parametrize("page", [16, 64, 1024])
+@pytest.mark.parametrize("order", ["hnd", "nhd", "mixed"])
+def test_prompt_pages_and_orders(gpu, page, order):
+    log(f"prompt page {page} {order}")
+    run_decode(gpu, Setup(8, 2, 128, page, "f16", [150, 65, 0, 31], [150, 7, 0, 30], order=order, seed=7))
+
+
+@pytest.mark.parametrize("heads", [(2, 1, 256), (4, 4, 64), (4, 1, 128)])
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_prompt_longer(gpu, heads, type):
+    log(f"prompt 700 rows {heads} {type}")
+    run_decode(gpu, Setup(*heads, 32, type, [700, 129], [700, 128], seed=8))
+
+
+@pytest.mark.parametrize("rows", [1, 3, 20])
+def test_prompt_few_rows_over_a_long_cache(gpu, rows):
+    log(f"prompt {rows} rows over 12000")
+    run_decode(gpu, Setup(4, 2, 128, 64, "bf16", [12000 + rows, rows], [rows, rows], seed=9))
+
+
+def test_prompt_of_one_row_each_equals_decode_in_bound(gpu):
+    import torch
+    log("prompt as decode")
+    kv = [5, 100, 33]
+    run_decode(gpu, Setup(*MODEL, 16, "f16", kv, [1, 1, 1], seed=10))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 3.0])
+@pytest.mark.parametrize("rows", [None, [40, 9]])
+def test_scales(gpu, scale, rows):
+    """scale 0 (all weights equal), negative, and large enough that one key takes nearly all."""
+    log(f"scale {scale} rows {rows}")
+    run_decode(gpu, Setup(8, 2, 64, 16, "f16", [150, 70], rows, seed=11), scale=scale)
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_small_weights_keep_their_bits(gpu, type):
+    """One key far above 3000 equal others that together outweigh it: e^-8.4 each."""
+    import torch
+    log(f"small weights {type}")
+    s = Setup(4, 1, 64, 16, type, [3001], seed=12)
+    s.q[:] = 1.0
+    s.K[0][:] = 0.0
+    s.K[0][1500] = 8.4 * 8 / 64
+    s.V[0][:] = torch.randn(3001, 1, 64, generator=torch.Generator().manual_seed(3)).abs().to(s.type)
+    run_decode(gpu, s)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_later_tokens_do_not_reach_earlier_rows(gpu, bad):
+    """A token whose key and value are not finite is seen by the rows from its own on only."""
+    import torch
+    log(f"prompt with {bad} at token 45 of 80")
+    s = Setup(8, 2, 128, 16, "bf16", [80], [80], seed=13)
+    want, bound, _, _ = s.reference()
+    s.V[0][45] = bad
+    s.K[0][45] = bad
+    o, _, flags = run_decode(gpu, s, ref=False)
+    check("o before", o[:45], want[:45], bound[:45])
+    assert torch.isnan(o[45:].float()).all() and flags == 0
+
+
+@pytest.mark.parametrize("heads", [(8, 2, 128), (4, 4, 64), (2, 1, 256)])
+def test_infinite_value_of_a_seen_token(gpu, heads):
+    """V_j = inf in some elements: those of the rows that see it are inf, all else stays in bound."""
+    import torch
+    log(f"inf value {heads}")
+    s = Setup(*heads, 16, "f16", [70], [70], seed=14)
+    want, bound, _, _ = s.reference()
+    s.V[0][30, :, 5] = float("inf")
+    o, _, _ = run_decode(gpu, s, ref=False)
+    assert (o[30:, :, 5] == math.inf).all()
+    o[30:, :, 5] = 0
+    want[30:, :, 5] = 0
+    check("o", o, want, bound)
+
+
+def test_minus_infinite_scores(gpu):
+    """A key of -inf has weight 0; a row whose every score is -inf gets 0, as one that sees nothing."""
+    import torch
+    log("-inf keys")
+    s = Setup(4, 2, 64, 16, "f16", [40], [40], seed=15)
+    s.q = s.q.abs() + 0.1
+    s.K[0][0] = float("-inf")
+    s.V[0][0] = 3.0
+    o, lse, _ = run_decode(gpu, s, ref=False)
+    assert (o[0] == 0).all() and (lse[0] == -math.inf).all()
+    t = Setup(4, 2, 64, 16, "f16", [40], [40], seed=15)
+    t.q = s.q
+    ref = Setup(4, 2, 64, 16, "f16", [39], [39], seed=15)
+    ref.q, ref.K, ref.V = s.q[1:], [s.K[0][1:]], [s.V[0][1:]]
+    want, bound, _, _ = ref.reference()
+    check("o", o[1:], want, bound)
+
+
+@pytest.mark.parametrize("rows", [None, [20, 9, 4]])
+def test_bad_pages_and_lengths_are_left_out_and_flagged(gpu, rows):
+    import torch
+    log(f"bad pages, rows {rows}")
+    s = Setup(8, 2, 64, 16, "f16", [100, 50, 30], rows, seed=16, pad_pages=0)
+    k, v = s.pools()
+    ctx = s.context(gpu)
+    call = ctx.attn_decode if rows is None else ctx.attn_prompt
+    cache, q = gpu.KVCache(k, v), s.q.cuda()
+    batch = s.seqs(gpu)
+    good = call(cache, batch, q).clone()
+    assert ctx.device_flags() == 0
+    # sequence 0 loses its page 2 (tokens 32..47)
+    for bad in (-1, s.n_pages, 2 ** 31 - 1, -2 ** 31):
+        batch.pages[0, 2] = bad
+        o = call(cache, batch, q)
+        assert ctx.device_flags() == gpu.DEVFLAG_BAD_PAGE
+        n0 = 1 if rows is None else rows[0]
+        assert torch.equal(o[n0:], good[n0:])
+        ref = Setup(8, 2, 64, 16, "f16", [84, 50, 30], rows, seed=16)
+        keep = list(range(32)) + list(range(48, 100))
+        ref.q, ref.K, ref.V = s.q, [s.K[0][keep]] + s.K[1:], [s.V[0][keep]] + s.V[1:]
+        want, bound, _, _ = ref.reference()
+        check("o", o[:n0], want[:n0], bound[:n0])
+    batch.pages[0, 2] = s.pages[0, 2].item()
+    # lengths out of range: below 0 is 0, behind the page list is the list's end
+    batch.kv_len[2] = -5
+    o = call(cache, batch, q)
+    assert ctx.device_flags() == gpu.DEVFLAG_BAD_SEQ
+    assert torch.equal(o[:-1 if rows is None else -4], good[:-1 if rows is None else -4])
+    assert (o[-1 if rows is None else -4:] == 0).all()
+    assert ctx.device_flags() == 0
+
+
+def test_length_behind_the_page_list(gpu):
+    import torch
+    log("length behind the list")
+    s = Setup(8, 2, 64, 16, "f16", [96, 50], seed=17, pad_pages=0)
+    k, v = s.pools()
+    ctx = s.context(gpu)
+    cache, batch, q = gpu.KVCache(k, v), s.seqs(gpu), s.q.cuda()
+    good = ctx.attn_decode(cache, batch, q)
+    batch.kv_len[0] = 2 ** 31 - 1
+    o = ctx.attn_decode(cache, batch, q)
+    assert ctx.device_flags() == gpu.DEVFLAG_BAD_SEQ
+    assert torch.equal(o, good)
+
+
+def test_row_start_that_does_not_ascend_touches_nothing_else(gpu):
+    """Every row written is one of the packed rows; nothing out of range is read or written."""
+    import torch
+    log("row_start not ascending")
+    s = Setup(4, 2, 64, 16, "bf16", [40, 40, 40, 40], [10, 10, 10, 10], seed=18)
+    k, v = s.pools()
+    ctx = s.context(gpu)
+    q = s.q.cuda()
+    for start in ([0, 30, 10, 50, 20], [-5, 10, 20, 30, 40], [0, 10, 20, 30, 2 ** 31 - 1], [40, 30, 20, 10, 0],
+                  [-2 ** 31, 0, 0, 0, 0]):
+        batch = s.seqs(gpu)
+        batch.row_start.copy_(torch.tensor(start, dtype=torch.int32))
+        buf = torch.full((s.n_rows + 20, 4, 64), 9.0, dtype=s.type, device="cuda")
+        ctx.attn_prompt(gpu.KVCache(k, v), batch, q, o=buf[10:-10])
+        ctx.device_flags()
+        assert (buf[:10] == 9.0).all() and (buf[-10:] == 9.0).all()
+
+
+@pytest.mark.parametrize("rows", [None, [30, 12]])
+def test_slices_of_wider_rows_and_output_in_place(gpu, rows):
+    """q and o as slices of wider rows (what lies beside them stays), and o in q's place."""
+    import torch
+    log(f"slices, rows {rows}")
+    s = Setup(8, 2, 128, 16, "f16", [90, 50], rows, seed=19)
+    want, bound, _, _ = s.reference()
+    k, v = s.pools()
+    ctx = s.context(gpu)
+    call = ctx.attn_decode if rows is None else ctx.attn_prompt
+    wide = torch.full((s.n_rows, 14, 128), 4.0, dtype=s.type, device="cuda")
+    wide[:, 2:10] = s.q.cuda()
+    out = torch.full((s.n_rows, 11, 128), 6.0, dtype=s.type, device="cuda")
+    call(gpu.KVCache(k, v), s.seqs(gpu), wide[:, 2:10], o=out[:, 1:9])
+    check("o", out[:, 1:9], want, bound)
+    assert (out[:, 0] == 6).all() and (out[:, 9:] == 6).all()
+    alone = out[:, 1:9].clone()
+    call(gpu.KVCache(k, v), s.seqs(gpu), wide[:, 2:10], o=wide[:, 2:10])
+    assert torch.equal(wide[:, 2:10], alone)
+    assert (wide[:, :2] == 4).all() and (wide[:, 10:] == 4).all()
+
+
+@pytest.mark.parametrize("rows", [None, [9, 130]])
+def test_same_bits_again(gpu, rows):
+    import torch
+    log(f"same bits, rows {rows}")
+    s = Setup(*MODEL, 16, "bf16", [4000, 1000], rows, seed=20)
+    k, v = s.pools()
+    ctx = s.context(gpu)
+    call = ctx.attn_decode if rows is None else ctx.attn_prompt
+    cache, batch, q = gpu.KVCache(k, v), s.seqs(gpu), s.q.cuda()
+    first = call(cache, batch, q)
+    for _ in range(10):
+        assert torch.equal(call(cache, batch, q), first)
+
+
+def test_offsets_past_32_bits(gpu):
+    """Pages that lie more than 2^32 bytes (and 2^31 elements) into the pools."""
+    import torch
+    log("pools of 5 GiB")
+    s = Setup(2, 1, 64, 1024, "f16", [1500, 40], [300, 40], seed=21)
+    small_k, small_v = s.pools()
+    n = 5 * 2 ** 30 // (1024 * 64 * 2)
+    k = torch.empty((n, 1, 1024, 64), dtype=torch.float16, device="cuda")
+    v = torch.empty_like(k)
+    far = [n - 1 - i * 3 for i in range(s.n_pages)]
+    for i, f in enumerate(far):
+        k[f], v[f] = small_k[i], small_v[i]
+    assert far[-1] * 1024 * 64 > 2 ** 31
+    want, bound, _, _ = s.reference()
+    batch = s.seqs(gpu)
+    for b, m in enumerate(s.kv):
+        for t in range(-(-m // 1024)):
+            batch.pages[b, t] = far[int(s.pages[b, t])]
+    ctx = s.context(gpu)
+    o = ctx.attn_prompt(gpu.KVCache(k, v), batch, s.q.cuda())
+    check("prompt", o, want, bound)
+    new = torch.randn((340, 1, 64), device="cuda")
+    ctx.kv_append(gpu.KVCache(k, v), batch, new, new + 1)
+    for t in (0, 299):
+        pos = 1200 + t
+        assert torch.equal(k[far[int(s.pages[0, pos // 1024])], 0, pos % 1024], new[t, 0].half())
+    dec = Setup(2, 1, 64, 1024, "f16", [1500, 40], seed=21)
+    ctx.kv_append(gpu.KVCache(k, v), batch, torch.cat([s.K[0][1200:], s.K[1]]).cuda(),
+                  torch.cat([s.V[0][1200:], s.V[1]]).cuda())
+    want, bound, _, _ = dec.reference()
+    o = ctx.attn_decode(gpu.KVCache(k, v), gpu.SeqBatch(batch.pages, batch.kv_len), dec.q.cuda())
+    check("decode", o, want, bound)
+    assert ctx.device_flags() == 0
+
+
+@pytest.mark.parametrize("src", ["same", "f32"])
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("order", ["hnd", "nhd", "mixed"])
+@pytest.mark.parametrize("heads", [MODEL, (12, 12, 64), (5, 5, 128)])
+def test_append(gpu, heads, order, type, src):
+    """Every new row lands in its place, rounded to nearest even; every other place stays."""
+    import torch
+    log(f"append {heads} {order} {type} {src}")
+    rows, before = [1, 0, 40, 3, 17], [0, 9, 5, 100, 15]
+    s = Setup(*heads, 16, type, [r + c for r, c in zip(rows, before)], rows, order=order, junk=7.0, seed=22,
+              extra_rows=2)
+    k, v = s.pools(filled=False)
+    hk = s.hkv
+    g = torch.Generator().manual_seed(5)
+    qkv = torch.randn((s.n_rows, s.hq + 2 * hk, s.d), generator=g)
+    # ties, values over the type's range, infinities and NaN
+    qkv[0, s.hq, :6] = torch.tensor([1 + 2.0 ** -11, 1 + 3 * 2.0 ** -9, 7e4, -3.4e38, float("inf"), float("nan")])
+    qkv = qkv if src == "f32" else qkv.to(s.type)
+    dev = qkv.cuda()
+    ctx = s.context(gpu)
+    ctx.kv_append(gpu.KVCache(k, v), s.seqs(gpu), dev[:, s.hq:s.hq + hk], dev[:, s.hq + hk:])
+    assert ctx.device_flags() == 0
+    wk, wv = torch.full((s.n_pages, hk, 16, s.d), 7.0, dtype=s.type), torch.full((s.n_pages, hk, 16, s.d), 7.0, dtype=s.type)
+    row = 0
+    for b, (r, c) in enumerate(zip(rows, before)):
+        for i in range(r):
+            pg, t = int(s.pages[b, (c + i) // 16]), (c + i) % 16
+            wk[pg, :, t] = qkv[row, s.hq:s.hq + hk].to(s.type)
+            wv[pg, :, t] = qkv[row, s.hq + hk:].to(s.type)
+            row += 1
+    for got, want in ((k, wk), (v, wv)):
+        got = got.cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(got.nan_to_num(nan=1.0), want.nan_to_num(nan=1.0))
+
+
+def test_append_decode_step(gpu):
+    """Without row_start every sequence's one row goes to its last place."""
+    import torch
+    log("append decode step")
+    s = Setup(8, 2, 64, 16, "f16", [1, 16, 17, 40], junk=0.0, seed=23)
+    k, v = s.pools(filled=False)
+    ctx = s.context(gpu)
+    nk, nv = torch.randn((4, 2, 64), device="cuda"), torch.randn((4, 2, 64), device="cuda")
+    ctx.kv_append(gpu.KVCache(k, v), s.seqs(gpu), nk, nv)
+    for b, n in enumerate(s.kv):
+        pg, t = int(s.pages[b, (n - 1) // 16]), (n - 1) % 16
+        assert torch.equal(k[pg, :, t], nk[b].half()) and torch.equal(v[pg, :, t], nv[b].half())
+        k[pg, :, t] = 0
+        v[pg, :, t] = 0
+    assert (k == 0).all() and (v == 0).all() and ctx.device_flags() == 0
+
+
+def test_append_out_of_range_is_left_out_and_flagged(gpu):
+    import torch
+    log("append out of range")
+    s = Setup(4, 2, 64, 16, "f16", [20, 20, 20], [4, 4, 4], junk=0.0, seed=24, pad_pages=0)
+    ctx = s.context(gpu)
+    nk = torch.ones((12, 2, 64), device="cuda")
+    for what, flag in (("page", gpu.DEVFLAG_BAD_PAGE), ("short", gpu.DEVFLAG_BAD_SEQ), ("long", gpu.DEVFLAG_BAD_SEQ)):
+        k, v = s.pools(filled=False)
+        batch = s.seqs(gpu)
+        if what == "page":
+            batch.pages[1, 1] = s.n_pages
+        elif what == "short":
+            batch.kv_len[1] = 0
+        else:
+            batch.kv_len[1] = 2 ** 31 - 1
+        ctx.kv_append(gpu.KVCache(k, v), batch, nk, nk)
+        assert ctx.device_flags() == flag, what
+        assert int((k != 0).sum()) == int((v != 0).sum()) == 8 * 2 * 64
+
+
+def test_captured_and_replayed(gpu):
+    """Append and both attentions in one graph, replayed as the sequences grow (the lengths and the
+    new rows are read from device memory), every replay against the eager calls."""
+    import torch
+    log("graph of append, prompt and decode")
+    hq, hkv, d, page = MODEL[0], MODEL[1], MODEL[2], 16
+    s = Setup(hq, hkv, d, page, "f16", [300, 40], junk=0.0, seed=25)
+    k, v = s.pools()
+    cache, batch = gpu.KVCache(k, v), s.seqs(gpu)
+    start = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    as_prompt = gpu.SeqBatch(batch.pages, batch.kv_len, start, n_rows=2)
+    ctx, other = s.context(gpu), s.context(gpu)
+    nk, nv = torch.randn((2, hkv, d), device="cuda"), torch.randn((2, hkv, d), device="cuda")
+    q = s.q.cuda()
+    o, p = torch.empty_like(q), torch.empty_like(q)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(st):
+        with torch.cuda.graph(g, stream=st):
+            ctx.kv_append(cache, batch, nk, nv)
+            ctx.attn_decode(cache, batch, q, o=o)
+            ctx.attn_prompt(cache, as_prompt, q, o=p)
+    torch.cuda.synchronize()
+    for step in range(5):
+        batch.kv_len.copy_(torch.tensor([max(1, 250 + 11 * step), 1 + 9 * step], dtype=torch.int32))
+        nk.normal_()
+        nv.normal_()
+        q.normal_()
+        o.fill_(float("nan"))
+        p.fill_(float("nan"))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, other.attn_decode(cache, batch, q)), step
+        assert torch.equal(p, other.attn_prompt(cache, as_prompt, q)), step
+        torch.cuda.synchronize()
+    assert ctx.device_flags() == 0
+
+
+def test_two_contexts_on_two_streams(gpu):
+    """Two contexts at work at once do not share anything."""
+    import torch
+    log("two streams")
+    s = Setup(*MODEL, 16, "bf16", [9000, 800], seed=26)
+    t = Setup(*MODEL, 16, "bf16", [500, 7000], seed=27)
+    got = []
+    for x in (s, t):
+        ctx = x.context(gpu)
+        cache, batch, q = gpu.KVCache(*x.pools()), x.seqs(gpu), x.q.cuda()
+        got.append((ctx, cache, batch, q, ctx.attn_decode(cache, batch, q)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [[], []]
+    for _ in range(20):
+        for i, (ctx, cache, batch, q, _) in enumerate(got):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(ctx.attn_decode(cache, batch, q))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in outs[i]:
+            assert torch.equal(o, got[i][4])
+
+
+def test_no_sequences_and_no_rows(gpu):
+    import torch
+    log("empty calls")
+    ctx = gpu.AttnContext(4, 2, 64, 16, 8)
+    k = torch.zeros((2, 2, 16, 64), dtype=torch.float16, device="cuda")
+    pages = torch.zeros((0, 3), dtype=torch.int32, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    q = torch.zeros((0, 4, 64), dtype=torch.float16, device="cuda")
+    empty = gpu.SeqBatch(pages, none)
+    assert ctx.attn_decode(gpu.KVCache(k, k.clone()), empty, q).shape == (0, 4, 64)
+    ctx.kv_append(gpu.KVCache(k, k.clone()), empty, q[:, :2], q[:, :2])
+    # a sequence without rows, and packed rows of no sequence
+    two = gpu.SeqBatch(torch.zeros((1, 3), dtype=torch.int32, device="cuda"),
+                       torch.ones(1, dtype=torch.int32, device="cuda"),
+                       torch.zeros(2, dtype=torch.int32, device="cuda"), n_rows=5)
+    o = torch.full((5, 4, 64), 3.0, dtype=torch.float16, device="cuda")
+    ctx.attn_prompt(gpu.KVCache(k, k.clone()), two, o.clone(), o=o)
+    assert (o == 3).all() and ctx.device_flags() == 0
+
+
+def test_a_layer_of_decode_steps_with_the_experts(gpu):
+    """A layer as it is used: a prompt in two pieces, then decode steps, each one append and attention,
+    and the layer's MoE FFN on the result -- against the attention of the whole text at once."""
+    import torch
+    log("prompt, decode steps and the FFN")
+    hq, hkv, d, page = 8, 2, 64, 16
+    H = hq * d
+    total, pieces, steps = 61, [30, 25], 6
+    s = Setup(hq, hkv, d, page, "f16", [total], [total], seed=28, junk=float("nan"))
+    want, bound, _, _ = s.reference()
+    k, v = s.pools(filled=False)
+    cache = gpu.KVCache(k, v)
+    ctx = s.context(gpu)
+    moe = gpu.Context(H, 256, 16, 1, 64, gpu.W_RENORM)
+    moe.bind_packed(0, gpu.gen_layer(H, 256, 16, 99))
+    K, V, Q = s.K[0].cuda(), s.V[0].cuda(), s.q.cuda()
+    pages = s.pages.cuda()
+    done, outs = 0, []
+    for n in pieces:
+        batch = gpu.SeqBatch(pages, torch.tensor([done + n], dtype=torch.int32, device="cuda"),
+                             torch.tensor([0, n], dtype=torch.int32, device="cuda"), n_rows=n)
+        ctx.kv_append(cache, batch, K[done:done + n], V[done:done + n])
+        outs.append(ctx.attn_prompt(cache, batch, Q[done:done + n]))
+        done += n
+    length = torch.tensor([done], dtype=torch.int32, device="cuda")
+    batch = gpu.SeqBatch(pages, length)
+    for _ in range(steps):
+        length += 1
+        ctx.kv_append(cache, batch, K[done:done + 1].float(), V[done:done + 1].float())
+        outs.append(ctx.attn_decode(cache, batch, Q[done:done + 1]))
+        done += 1
+    o = torch.cat(outs)
+    check("o", o, want, bound)
+    assert ctx.device_flags() == 0
+    # the FFN of every row of the attention's output equals that of the whole output at once
+    x = o.float().view(total, H)
+    logits = gpu.gen_logits(total, 16, 7)
+    whole, _, _ = moe.ffn_route(0, x, logits, rmsnorm=True)
+    last, _, _ = moe.ffn_route(0, x[-1:].contiguous(), logits[-1:].contiguous(), rmsnorm=True)
+    torch.cuda.synchronize()
+    err = (whole[-1] - last[0]).abs().max() / whole[-1].abs().max()
+    assert err <= 1e-3 + 5e-3  # the two paths' own bounds against the FFN's definition
+    moe.close()
+
+
+def test_refusals(gpu):
+    """What a call refuses on the host, with a live handle: the C entry's statuses, then the binding's."""
+    import ctypes
+    import torch
+    L = gpu.lib()
+    ctx = gpu.AttnContext(4, 2, 64, 16, 4)
+    k = torch.zeros((3, 2, 16, 64), dtype=torch.float16, device="cuda")
+    v = torch.zeros_like(k)
+    pages = torch.zeros((2, 3), dtype=torch.int32, device="cuda")
+    lens = torch.ones(2, dtype=torch.int32, device="cuda")
+    start = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    q = torch.zeros((2, 4, 64), dtype=torch.float16, device="cuda")
+    o = torch.zeros_like(q)
+    cache, batch, packed = gpu.KVCache(k, v), gpu.SeqBatch(pages, lens), gpu.SeqBatch(pages, lens, start, n_rows=2)
+    st = torch.cuda.current_stream().cuda_stream
+
+    def decode(kv=None, s=None, q_=q.data_ptr(), qs=256, scale=0.1, o_=o.data_ptr(), os=256, lse=None, fn=None):
+        kv, s = cache._c if kv is None else kv, batch._c if s is None else s
+        return (fn or L.moe_attn_decode)(ctx.handle, ctypes.addressof(kv), ctypes.addressof(s), q_, qs, scale, o_, os,
+                                         lse, st)
+
+    def changed(struct, **kw):
+        c = type(struct)()
+        ctypes.pointer(c)[0] = struct
+        for n, val in kw.items():
+            setattr(c, n, val)
+        return c
+
+    EINVAL = gpu.MOE_EINVAL
+    assert decode() == gpu.MOE_OK
+    assert decode(s=packed._c) == EINVAL  # row_start in a decode call
+    assert decode(s=packed._c, fn=L.moe_attn_prompt) == gpu.MOE_OK
+    for kw in (dict(q_=None), dict(o_=None), dict(qs=248), dict(os=255), dict(qs=260), dict(scale=float("nan")),
+               dict(scale=float("inf")), dict(q_=q.data_ptr() + 8), dict(o_=o.data_ptr() + 2), dict(lse=o.data_ptr() + 2),
+               dict(o_=q.data_ptr(), os=264)):
+        assert decode(**kw) == EINVAL, kw
+        assert L.moe_last_error()
+    for kw in (dict(k=None), dict(v=None), dict(k=k.data_ptr() + 8), dict(n_pages=0), dict(page_stride=0),
+               dict(head_stride=-64), dict(token_stride=32), dict(token_stride=68), dict(page_stride=1 << 50)):
+        assert decode(kv=changed(cache._c, **kw)) == EINVAL, kw
+    for kw in (dict(n_seqs=-1), dict(n_seqs=5), dict(n_rows=3), dict(n_rows=-1), dict(pages=None), dict(kv_len=None),
+               dict(pages=pages.data_ptr() + 2), dict(max_pages=0), dict(pages_stride=2), dict(max_pages=1 << 30)):
+        assert decode(s=changed(batch._c, **kw)) == EINVAL, kw
+    assert decode(s=changed(packed._c, n_rows=(1 << 24) + 1), fn=L.moe_attn_prompt) == EINVAL
+    new = torch.zeros((2, 2, 64), device="cuda")
+
+    def append(t=gpu.T_F32, ks=128, vs=128, kp=new.data_ptr(), vp=new.data_ptr()):
+        return L.moe_kv_append(ctx.handle, cache._ref, batch._ref, kp, vp, t, ks, vs, st)
+
+    assert append() == gpu.MOE_OK
+    assert append(t=gpu.T_BF16) == gpu.MOE_EUNSUPPORTED and append(t=5) == gpu.MOE_EUNSUPPORTED
+    for kw in (dict(ks=124), dict(vs=130), dict(kp=None), dict(vp=None), dict(kp=new.data_ptr() + 4)):
+        assert append(**kw) == EINVAL, kw
+    assert L.moe_attn_flags(ctx.handle, st, None) == EINVAL
+    assert L.moe_attn_flags_async(ctx.handle, lens.data_ptr() + 1, st) == EINVAL
+    out = ctypes.c_void_p()
+    assert L.moe_attn_create(99, ctypes.byref(gpu._AttnConfig(4, 2, 64, 16, 1, 4)), ctypes.byref(out)) == EINVAL
+    # the binding
+    cpu = torch.zeros((2, 4, 64), dtype=torch.float16)
+    other = torch.zeros((3, 2, 32, 64), dtype=torch.float16, device="cuda")
+    for bad in (lambda: ctx.attn_decode(cache, batch, cpu), lambda: ctx.attn_decode(cache, batch, q.bfloat16()),
+                lambda: ctx.attn_decode(cache, batch, q[:1]), lambda: ctx.attn_decode(cache, batch, q[:, :3]),
+                lambda: ctx.attn_decode(cache, batch, q, o=o.float()), lambda: ctx.attn_decode(cache, batch, q, o=o[:, :, :32]),
+                lambda: ctx.attn_decode(cache, batch, q.transpose(1, 2).contiguous().transpose(1, 2)),
+                lambda: ctx.attn_decode(cache, batch, q, lse=torch.zeros(2, 4)),
+                lambda: ctx.attn_decode(cache, batch, q, lse=torch.zeros((2, 4), dtype=torch.float64, device="cuda")),
+                lambda: ctx.attn_decode(gpu.KVCache(other, other), batch, q),
+                lambda: ctx.attn_decode(gpu.KVCache(k.bfloat16(), v.bfloat16()), batch, q),
+                lambda: ctx.attn_decode(gpu.KVCache(k.cpu(), v.cpu()), batch, q),
+                lambda: ctx.attn_decode(cache, gpu.SeqBatch(pages.cpu(), lens.cpu()), q),
+                lambda: ctx.kv_append(cache, batch, new, new.half()), lambda: ctx.kv_append(cache, batch, new.bfloat16(), new.bfloat16()),
+                lambda: ctx.kv_append(cache, batch, new.cpu(), new.cpu()), lambda: ctx.kv_append(cache, batch, new[:1], new)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(gpu.MoeError):
+        ctx.attn_decode(cache, packed, q)
+    dst = torch.zeros(1, dtype=torch.int32, device="cuda")
+    lens[0] = -1
+    ctx.attn_decode(cache, batch, q)
+    ctx.device_flags_async(dst)
+    assert dst.item() == gpu.DEVFLAG_BAD_SEQ and ctx.device_flags() == 0
+    ctx.close()
+    with pytest.raises(ValueError):
+        ctx.attn_decode(cache, batch, q)
