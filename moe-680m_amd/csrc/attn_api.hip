@@ -15,6 +15,10 @@ struct moe_attn {
     int page_shift = 0;
     void *arena = nullptr;     // one device allocation, carved below
     uint32_t *flags = nullptr; // sticky device flags
+    float *part = nullptr;     // decode partials: [2 n_wg][DEC_HEADS][head_dim]
+    float *part_ml = nullptr;  // [2 n_wg][DEC_HEADS][2]
+    uint32_t *arrived = nullptr; // [n_wg], zero between calls
+    int n_wg = 0;              // workgroups of a decode launch
 };
 
 namespace {
@@ -64,8 +68,8 @@ moe_status common_args(const char *fn, moe_attn *a, const moe_kv_cache *kv, cons
     if (kv->n_pages < 1) return fail(MOE_EINVAL, "%s: a cache of %d pages", fn, kv->n_pages);
     const int64_t strides[3] = {kv->page_stride, kv->head_stride, kv->token_stride};
     for (int64_t v : strides)
-        if (v < g.head_dim || (v & 7) || v > ((int64_t)1 << 40))
-            return fail(MOE_EINVAL, "%s: cache stride %lld (multiples of 8 elements, head_dim=%d at least)", fn,
+        if (v < g.head_dim || (v & 7) || v > ((int64_t)1 << 40) || kv->token_stride > (1 << 24))
+            return fail(MOE_EINVAL, "%s: cache stride %lld (multiples of 8, head_dim=%d at least; token_stride at most 2^24)", fn,
                         (long long)v, g.head_dim);
     *c = AttnArgs{};
     if (s->n_seqs == 0 || s->n_rows == 0) return MOE_OK; // nothing to do: no other pointer is needed
@@ -115,9 +119,15 @@ moe_status attn_call(const char *fn, moe_attn *a, const moe_kv_cache *kv, const 
     c.o_stride = o_stride;
     c.lse = lse;
     c.scale_log2 = (float)(scale * 1.4426950408889634);
+    c.part = a->part;
+    c.part_ml = a->part_ml;
+    c.arrived = a->arrived;
+    c.n_wg = a->n_wg;
     OnDevice on(a->device);
     hipError_t he = on.he;
-    if (he == hipSuccess) he = launch_attn(c, a->cfg.type, a->cfg.head_dim, (hipStream_t)stream);
+    if (he == hipSuccess)
+        he = c.row_start ? launch_attn(c, a->cfg.type, a->cfg.head_dim, (hipStream_t)stream)
+                         : launch_attn_decode(c, a->cfg.type, a->cfg.head_dim, (hipStream_t)stream);
     if (he != hipSuccess) return fail(MOE_EHIP, "%s: launch: %s", fn, hipGetErrorString(he));
     return ok();
 }
@@ -152,14 +162,31 @@ moe_status moe_attn_create(int device, const moe_attn_config *cfg, moe_attn **ou
     a->device = device;
     a->cfg = g;
     while ((1 << a->page_shift) < g.page_tokens) ++a->page_shift;
-    const size_t total = 256;
+    int ncu = 0;
+    if (hipDeviceGetAttribute(&ncu, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || ncu < 1) ncu = 1;
+    a->n_wg = 2 * ncu;
+    struct Part {
+        void **dst;
+        size_t bytes;
+    } parts[] = {
+        {(void **)&a->flags, 256},
+        {(void **)&a->arrived, (size_t)a->n_wg * 4},
+        {(void **)&a->part_ml, (size_t)a->n_wg * 2 * DEC_HEADS * 2 * 4},
+        {(void **)&a->part, (size_t)a->n_wg * 2 * DEC_HEADS * g.head_dim * 4},
+    };
+    size_t total = 0;
+    for (auto &p : parts) total += (p.bytes + 255) / 256 * 256;
     he = hipMalloc(&a->arena, total);
     if (he != hipSuccess) {
         (void)hipGetLastError();
         delete a;
         return fail(MOE_ENOMEM, "%s: hipMalloc(%zu): %s", fn, total, hipGetErrorString(he));
     }
-    a->flags = (uint32_t *)a->arena;
+    size_t off = 0;
+    for (auto &p : parts) {
+        *p.dst = (char *)a->arena + off;
+        off += (p.bytes + 255) / 256 * 256;
+    }
     he = hipMemset(a->arena, 0, total);
     if (he == hipSuccess) he = hipDeviceSynchronize();
     if (he != hipSuccess) {

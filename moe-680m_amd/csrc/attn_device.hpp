@@ -1,0 +1,68 @@
+// attn_device.hpp -- device helpers of the attention kernels.
+#pragma once
+
+#include "attn_internal.hpp"
+#include "moe_device.hpp"
+
+namespace moe {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
+
+// Softmax weights meet the values in the cache's type.  They are taken relative to the running
+// maximum and, for f16, 2^15 above it: f16 keeps all its bits down to 2^-14, so a weight loses bits
+// only below 2^-29 of the largest (unshifted below 2^-14, where thousands of such keys can hold most
+// of the mass).  bf16 has f32's range.
+template <typename T>
+struct Elem;
+template <>
+struct Elem<f16_t> {
+    typedef f16x8 x8;
+    static constexpr float SHIFT = 15.f;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
+    }
+    static __device__ __forceinline__ f32x4 mfma16(x8 a, x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(x8 a, x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Elem<bf16_t> {
+    typedef bf16x8 x8;
+    static constexpr float SHIFT = 0.f;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+    }
+    static __device__ __forceinline__ f32x4 mfma16(x8 a, x8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(x8 a, x8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// The maximum to subtract: 0 while no score was seen (every score -inf: all weights 0).
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+__device__ __forceinline__ void raise(uint32_t *flags, uint32_t bit) {
+    __hip_atomic_fetch_or((MOE_GLOBAL uint32_t *)flags, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// A load from an address that is the same in all lanes, of memory that no launch under way writes:
+// through the scalar cache, so it waits for no vector load in flight.
+template <typename T>
+__device__ __forceinline__ T ldc(const T *p) {
+    return *(const __attribute__((address_space(4))) T *)p;
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+} // namespace moe

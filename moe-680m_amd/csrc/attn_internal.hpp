@@ -24,7 +24,17 @@ struct AttnArgs {
     int n_seqs, n_rows;
     int hq, hkv, group;       // group = hq / hkv
     float scale_log2;         // scale * log2(e): exponentials are taken in base 2
+    float *part;              // workspace: partial rows of pieces (see k_attn_decode.hip)
+    float *part_ml;           // ... and each partial row's running maximum and sum
+    uint32_t *arrived;        // ... and the pieces that have arrived (zero between calls)
+    int n_wg;                 // workgroups of a decode launch
 };
+
+// Decode: heads of one matrix tile, tokens of one workgroup step and of one wave's.
+constexpr int DEC_HEADS = 16;
+constexpr int DEC_WAVES = 4;
+constexpr int DEC_WAVE_TOK = 32;
+constexpr int DEC_TILE = DEC_WAVES * DEC_WAVE_TOK;
 
 struct AppendArgs {
     const uint8_t *src[2];    // new keys, new values
@@ -34,6 +44,7 @@ struct AppendArgs {
 };
 
 hipError_t launch_kv_append(const AppendArgs &a, int type, int in_type, int d, hipStream_t st);
+hipError_t launch_attn_decode(const AttnArgs &a, int type, int d, hipStream_t st);
 hipError_t launch_attn(const AttnArgs &a, int type, int d, hipStream_t st);
 hipError_t launch_attn_flags(uint32_t *flags, uint32_t *dst, hipStream_t st);
 

@@ -1,0 +1,341 @@
+// k_attn_decode.hip -- one new token of every sequence over its paged cache.
+//
+//   o[h] = sum_j e^(s_j - m) V_j / sum_j e^(s_j - m),   s_j = scale * q[h] . K_j
+//
+// Bound by reading K and V once (4 bytes of K and V for 4 * group operations a head element, far
+// below the matrix rate), so all that matters is to keep every CU's loads in flight:
+//
+//   * Work is cut by the lengths as they are in device memory, not by the host's bound: a tile is
+//     DEC_TILE tokens of one (sequence, key-value head, 16 query heads), tiles are numbered
+//     through, and each of the n_wg resident workgroups takes an equal run of them.  A run that
+//     ends inside a sequence leaves a partial row (maximum, sum, unnormalised output); the last
+//     workgroup of a sequence to arrive joins its partials in their order (same bits every time).
+//   * A wave takes 32 tokens of a tile by itself, no barrier until the run leaves the sequence:
+//       S^T[token][head] = K Q^T       16x16x32 products, A rows = tokens straight from memory
+//                                      (a lane's 16 bytes = 8 elements of one token)
+//       O^T[d][head] += V^T P^T        B = P^T is S^T's own register layout: lane (head, g) holds
+//                                      tokens 4g..4g+3 and 16+4g..16+4g+3, and V's tokens are taken in
+//                                      that order, so P never moves between lanes
+//     V^T: a lane loads 8 tokens x 8 consecutive elements (whole rows are contiguous over 16
+//     lanes) and swaps them in registers, two v_perm a dword pair; the matrix row m of product j
+//     is element 8 m + j, which only the output's addressing sees.
+//   * A wave's loads of the next 32 tokens' K are issued before the softmax, those of V after the
+//     products: some 16 KB a wave are always under way.
+#include "attn_device.hpp"
+
+namespace moe {
+
+namespace {
+
+// Tiles of a sequence: one at least, so that an empty one's row is written too.
+__device__ __forceinline__ int seq_tiles(const AttnArgs &a, int b, int cap) {
+    const int n = min(max(a.kv_len[b], 0), cap);
+    return max(1, (n + DEC_TILE - 1) / DEC_TILE);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
+    typedef Elem<T> E;
+    typedef typename E::x8 x8;
+    constexpr int KS = D / 32;               // products of a score tile
+    constexpr int VW = D >= 128 ? 8 : 4;     // elements of a lane's V load
+    constexpr int VS = D / (16 * VW);        // loads a token
+    typedef uint32_t vload __attribute__((ext_vector_type(VW / 2)));
+    __shared__ float s_o[DEC_WAVES][DEC_HEADS][D];
+    __shared__ float s_ml[DEC_WAVES][DEC_HEADS][2];
+    __shared__ uint32_t s_scan[DEC_WAVES], s_find[2];
+    __shared__ uint32_t s_last;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int c = lane & 15, g = lane >> 4;
+    const int cap = a.max_pages << a.page_shift;
+    const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS, hb_n = a.hkv * gb;
+
+    // ---- this workgroup's run of tiles [lo, hi): prefix sums over the sequences
+    const int per = (a.n_seqs + 255) / 256;
+    uint32_t mine = 0;
+    for (int i = 0; i < per; ++i) {
+        const int b = tid * per + i;
+        if (b < a.n_seqs) mine += (uint32_t)seq_tiles(a, b, cap);
+    }
+    uint32_t incl = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t v = __shfl_up(incl, o);
+        if (lane >= o) incl += v;
+    }
+    if (lane == 63) s_scan[wave] = incl;
+    __syncthreads();
+    uint32_t before = 0, total_seq = 0;
+    for (int w = 0; w < DEC_WAVES; ++w) {
+        if (w < wave) before += s_scan[w];
+        total_seq += s_scan[w];
+    }
+    before += incl - mine;
+    const uint64_t total = (uint64_t)total_seq * hb_n;
+    const uint32_t share = (uint32_t)((total + gridDim.x - 1) / gridDim.x);
+    const uint64_t lo = (uint64_t)blockIdx.x * share;
+    if (lo >= total) return;
+    const uint64_t hi = lo + share < total ? lo + share : total;
+    {
+        const uint64_t first = (uint64_t)before * hb_n;
+        if (first <= lo && lo < first + (uint64_t)mine * hb_n) {
+            uint32_t p = before;
+            int b = tid * per;
+            for (;; ++b) {
+                const uint32_t n = (uint32_t)seq_tiles(a, b, cap);
+                if (lo < (uint64_t)(p + n) * hb_n) break;
+                p += n;
+            }
+            s_find[0] = (uint32_t)b;
+            s_find[1] = p;
+        }
+    }
+    __syncthreads();
+    int b = uniform((int)s_find[0]);
+    uint64_t at = (uint64_t)(uint32_t)uniform((int)s_find[1]) * hb_n; // first tile of sequence b
+    int nt = uniform(seq_tiles(a, b, cap));
+    int hb = (int)((lo - at) / (uint32_t)nt);
+    uint64_t unit = at + (uint64_t)hb * nt; // first tile of (b, hb)
+
+    for (uint64_t pos = lo; pos < hi;) {
+        const int t0 = (int)(pos - unit);
+        const int t1 = (int)((hi < unit + nt ? hi : unit + nt) - unit);
+        const int len = ldc(a.kv_len + b);
+        const int seen = min(max(len, 0), cap);
+        if (seen != len && tid == 0) raise(a.flags, MOE_DEVFLAG_BAD_SEQ);
+        const int hk = hb / gb, h0 = hk * a.group + (hb - hk * gb) * DEC_HEADS;
+        const int nh = min(DEC_HEADS, (hk + 1) * a.group - h0); // heads of this unit
+        const T *q = (const T *)a.q + b * a.q_stride + (int64_t)(h0 + min(c, nh - 1)) * D;
+        x8 qf[KS];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) qf[k] = ldg<x8>(q + k * 32 + g * 8);
+
+        f32x4 acc[D / 16];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+        const int32_t *pages = a.pages + b * a.pages_stride;
+        const uint8_t *kb = a.k + 2 * hk * a.head_stride, *vb = a.v + 2 * hk * a.head_stride;
+        const int ts2 = (int)(2 * a.token_stride);
+        const int mask = (1 << a.page_shift) - 1;
+        const int end = min(seen, t1 * DEC_TILE); // of this piece
+        bool bad = false;
+
+        // the two 16-token halves of a step: byte offset of the first token, tokens there
+        int64_t off[2];
+        int have[2];
+        auto place = [&](int tok) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int t = tok + 16 * i;
+                have[i] = min(16, end - t);
+                int pg = 0;
+                if (have[i] > 0) {
+                    pg = ldc(pages + (t >> a.page_shift));
+                    if ((unsigned)pg >= (unsigned)a.n_pages) bad = true, pg = 0, have[i] = 0;
+                } else have[i] = 0;
+                off[i] = 2 * (pg * a.page_stride + (t & mask) * a.token_stride);
+            }
+        };
+        x8 kf[2][KS];
+        vload vf[8][VS];
+        // a lane whose token is not there reads the last one that is (the first place if none is)
+        auto load_k = [&]() {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint8_t *p = kb + off[i] + max(0, min(c, have[i] - 1)) * ts2 + g * 16;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) kf[i][k] = ldg<x8>(p + k * 64);
+            }
+        };
+        auto load_v = [&](const int64_t *off, const int *have) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = j >> 2, t = max(0, min(4 * g + (j & 3), have[i] - 1));
+                const uint8_t *p = vb + off[i] + t * ts2 + c * (VW * 2);
+#pragma unroll
+                for (int s = 0; s < VS; ++s) vf[j][s] = ldg<vload>(p + s * (32 * VW));
+            }
+        };
+        int tok = t0 * DEC_TILE + wave * DEC_WAVE_TOK;
+        if (tok < end) {
+            place(tok);
+            load_k();
+            load_v(off, have);
+        }
+        for (; tok < end; tok += DEC_TILE) {
+            const int hv[2] = {have[0], have[1]};
+            f32x4 st[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                st[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KS; ++k) st[i] = E::mfma16(kf[i][k], qf[k], st[i]);
+            }
+            const bool more = tok + DEC_TILE < end;
+            int64_t nx_off[2] = {off[0], off[1]};
+            if (more) {
+                place(tok + DEC_TILE);
+                load_k();
+                nx_off[0] = off[0];
+                nx_off[1] = off[1];
+            }
+            float mx = m;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    st[i][r] = 4 * g + r < hv[i] ? st[i][r] * a.scale_log2 : -INFINITY;
+                    mx = fmaxf(mx, st[i][r]);
+                }
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float mb = base_of(mx);
+            const float alpha = exp2_(m - mb);
+            m = mx;
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = exp2_(st[i >> 2][i & 3] - (mb - E::SHIFT));
+            l = l * alpha + (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7])));
+            const u32x4 pw = {E::pack(p[0], p[1]), E::pack(p[2], p[3]), E::pack(p[4], p[5]), E::pack(p[6], p[7])};
+            const x8 pf = __builtin_bit_cast(x8, pw);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) acc[i] *= alpha;
+            if (hv[0] < 16 || hv[1] < 16) { // values that are not seen: 0 (0 * inf would be NaN)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (4 * g + (j & 3) >= hv[j >> 2])
+#pragma unroll
+                        for (int s = 0; s < VS; ++s) vf[j][s] = vload{};
+            }
+#pragma unroll
+            for (int s = 0; s < VS; ++s)
+#pragma unroll
+                for (int w = 0; w < VW / 2; ++w) {
+                    u32x4 e0, e1;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        e0[i] = __builtin_amdgcn_perm(vf[2 * i + 1][s][w], vf[2 * i][s][w], 0x05040100u);
+                        e1[i] = __builtin_amdgcn_perm(vf[2 * i + 1][s][w], vf[2 * i][s][w], 0x07060302u);
+                    }
+                    f32x4 &a0 = acc[s * VW + 2 * w], &a1 = acc[s * VW + 2 * w + 1];
+                    a0 = E::mfma16(__builtin_bit_cast(x8, e0), pf, a0);
+                    a1 = E::mfma16(__builtin_bit_cast(x8, e1), pf, a1);
+                }
+            if (more) load_v(nx_off, have);
+        }
+        if (bad && lane == 0) raise(a.flags, MOE_DEVFLAG_BAD_PAGE);
+
+        // ---- join the four waves: row (head c) of O^T's register layout to s_o[wave][head][d]
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        if (g == 0) {
+            s_ml[wave][c][0] = m;
+            s_ml[wave][c][1] = l;
+        }
+        // the row's elements 16 VW s + VW (4 g + r) + j, j = 0..VW-1
+#pragma unroll
+        for (int s = 0; s < VS; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int j = 0; j < VW; j += 4)
+                    *(f32x4 *)&s_o[wave][c][16 * VW * s + VW * (4 * g + r) + j] =
+                        f32x4{acc[s * VW + j][r], acc[s * VW + j + 1][r], acc[s * VW + j + 2][r], acc[s * VW + j + 3][r]};
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == nt;
+        const uint32_t slot = 2 * blockIdx.x + (t0 == 0 ? 1u : 0u);
+        constexpr int PER = DEC_HEADS * D / 256; // elements a thread: one head's, consecutive
+        const int hh = tid * PER / D, d0 = tid * PER % D;
+        float M = -INFINITY, f[DEC_WAVES], L = 0.f, x[PER];
+#pragma unroll
+        for (int w = 0; w < DEC_WAVES; ++w) M = fmaxf(M, s_ml[w][hh][0]);
+#pragma unroll
+        for (int w = 0; w < DEC_WAVES; ++w) {
+            f[w] = exp2_(s_ml[w][hh][0] - base_of(M));
+            L += f[w] * s_ml[w][hh][1];
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < DEC_WAVES; ++w)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) x[i] += f[w] * s_o[w][hh][d0 + i];
+        bool write = whole;
+        if (!whole) {
+            if (hh < nh) {
+                float *po = a.part + ((size_t)slot * DEC_HEADS + hh) * D + d0;
+#pragma unroll
+                for (int i = 0; i < PER; i += 4) *(f32x4 *)(po + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+                if (d0 == 0) *(f32x2 *)(a.part_ml + ((size_t)slot * DEC_HEADS + hh) * 2) = f32x2{M, L};
+            }
+            // the pieces of this unit: workgroups w0 (its tail slot) to w1 (their head slots)
+            const uint32_t w0 = (uint32_t)(unit / share), w1 = (uint32_t)((unit + nt - 1) / share);
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) s_last = atomicAdd(a.arrived + w0, 1u);
+            __syncthreads();
+            if (s_last == w1 - w0) {
+                __threadfence();
+                write = true;
+                if (tid == 0) a.arrived[w0] = 0;
+                M = -INFINITY;
+                L = 0.f;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) x[i] = 0.f;
+                if (hh < nh)
+                    for (uint32_t w = w0; w <= w1; ++w) {
+                        const size_t sl = ((size_t)(2 * w + (w == w0 ? 1u : 0u)) * DEC_HEADS + hh);
+                        const f32x2 ml = *(const f32x2 *)(a.part_ml + sl * 2);
+                        const float mx = fmaxf(M, ml.x), fo = exp2_(M - base_of(mx)), fn = exp2_(ml.x - base_of(mx));
+                        M = mx;
+                        L = L * fo + ml.y * fn;
+                        const float *po = a.part + sl * D + d0;
+#pragma unroll
+                        for (int i = 0; i < PER; i += 4) {
+                            const f32x4 v = *(const f32x4 *)(po + i);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) x[i + j] = x[i + j] * fo + v[j] * fn;
+                        }
+                    }
+            }
+        }
+        if (write && hh < nh) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            T *o = (T *)a.o + b * a.o_stride + (int64_t)(h0 + hh) * D + d0;
+#pragma unroll
+            for (int i = 0; i < PER; i += 2)
+                *(uint32_t *)(o + i) = E::pack(L == 0.f ? 0.f : x[i] * inv, L == 0.f ? 0.f : x[i + 1] * inv);
+            if (a.lse && d0 == 0)
+                a.lse[(int64_t)b * a.hq + h0 + hh] =
+                    L == 0.f ? -INFINITY : (base_of(M) - E::SHIFT + __log2f(L)) * 0.69314718055994531f;
+        }
+        pos = unit + t1;
+        if (pos < hi) { // the next (sequence, heads)
+            __syncthreads(); // s_o is free again
+            unit += nt;
+            if (++hb == hb_n) {
+                hb = 0;
+                ++b;
+                nt = uniform(seq_tiles(a, b, cap));
+            }
+        }
+    }
+}
+
+template <typename T>
+hipError_t decode_d(const AttnArgs &a, int d, hipStream_t st) {
+    const unsigned grid = (unsigned)a.n_wg;
+    if (d == 64) k_attn_decode<T, 64><<<grid, 256, 0, st>>>(a);
+    else if (d == 128) k_attn_decode<T, 128><<<grid, 256, 0, st>>>(a);
+    else k_attn_decode<T, 256><<<grid, 256, 0, st>>>(a);
+    return hipGetLastError();
+}
+
+} // namespace
+
+hipError_t launch_attn_decode(const AttnArgs &a, int type, int d, hipStream_t st) {
+    return type == MOE_T_F16 ? decode_d<f16_t>(a, d, st) : decode_d<bf16_t>(a, d, st);
+}
+
+} // namespace moe
