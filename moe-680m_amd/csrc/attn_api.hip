@@ -15,9 +15,9 @@ struct moe_attn {
     int page_shift = 0;
     void *arena = nullptr;     // one device allocation, carved below
     uint32_t *flags = nullptr; // sticky device flags
-    float *part = nullptr;     // decode partials: [2 n_wg][DEC_HEADS][head_dim]
-    float *part_ml = nullptr;  // [2 n_wg][DEC_HEADS][2]
-    uint32_t *arrived = nullptr; // [n_wg], zero between calls
+    float *part = nullptr;     // decode partials: [2 n_wg][DEC_WAVES][DEC_HEADS][head_dim]
+    float *part_ml = nullptr;  // [2 n_wg][DEC_WAVES][DEC_HEADS][2]
+    uint32_t *arrived = nullptr; // [3 n_wg], zero between calls
     int n_wg = 0;              // workgroups of a decode launch
 };
 
@@ -164,15 +164,15 @@ moe_status moe_attn_create(int device, const moe_attn_config *cfg, moe_attn **ou
     while ((1 << a->page_shift) < g.page_tokens) ++a->page_shift;
     int ncu = 0;
     if (hipDeviceGetAttribute(&ncu, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || ncu < 1) ncu = 1;
-    a->n_wg = 2 * ncu;
+    a->n_wg = 2 * ncu < DEC_MAX_WG ? 2 * ncu : DEC_MAX_WG;
     struct Part {
         void **dst;
         size_t bytes;
     } parts[] = {
         {(void **)&a->flags, 256},
-        {(void **)&a->arrived, (size_t)a->n_wg * 4},
-        {(void **)&a->part_ml, (size_t)a->n_wg * 2 * DEC_HEADS * 2 * 4},
-        {(void **)&a->part, (size_t)a->n_wg * 2 * DEC_HEADS * g.head_dim * 4},
+        {(void **)&a->arrived, (size_t)a->n_wg * 3 * 4},
+        {(void **)&a->part_ml, (size_t)a->n_wg * 2 * DEC_WAVES * DEC_HEADS * 2 * 4},
+        {(void **)&a->part, (size_t)a->n_wg * 2 * DEC_WAVES * DEC_HEADS * g.head_dim * 4},
     };
     size_t total = 0;
     for (auto &p : parts) total += (p.bytes + 255) / 256 * 256;

@@ -63,6 +63,26 @@ __device__ __forceinline__ T ldc(const T *p) {
     return *(const __attribute__((address_space(4))) T *)p;
 }
 
+// Partial rows that workgroups on other XCDs (each with an L2 of its own) join: stored at agent scope,
+// which writes through the producer's L2, and read at system scope, past the reader's.  A
+// workgroup's barrier waits for its stores, so a count added behind the barrier says that they are
+// there.  Fences in their place write back and invalidate whole L2s: 10 us and more a join.
+__device__ __forceinline__ void publish(float *p, f32x2 v) {
+    __hip_atomic_store((MOE_GLOBAL uint64_t *)p, __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void publish(float *p, f32x4 v) {
+    publish(p, f32x2{v[0], v[1]});
+    publish(p + 2, f32x2{v[2], v[3]});
+}
+__device__ __forceinline__ f32x4 remote4(const float *p) {
+    return __builtin_bit_cast(f32x4, remote_quad((const u32x4 *)p));
+}
+__device__ __forceinline__ f32x2 remote2(const float *p) {
+    return __builtin_bit_cast(f32x2, __hip_atomic_load((const MOE_GLOBAL uint64_t *)p, __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_SYSTEM));
+}
+
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 } // namespace moe

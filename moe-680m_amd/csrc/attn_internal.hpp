@@ -26,15 +26,16 @@ struct AttnArgs {
     float scale_log2;         // scale * log2(e): exponentials are taken in base 2
     float *part;              // workspace: partial rows of pieces (see k_attn_decode.hip)
     float *part_ml;           // ... and each partial row's running maximum and sum
-    uint32_t *arrived;        // ... and the pieces that have arrived (zero between calls)
+    uint32_t *arrived;        // ... and counts of the pieces that have arrived (zero between calls)
     int n_wg;                 // workgroups of a decode launch
+    int wpu_shift;            // decode: log2 of the waves that share a unit
 };
 
-// Decode: heads of one matrix tile, tokens of one workgroup step and of one wave's.
+// Decode: heads of one matrix tile, waves of a workgroup, tokens of a wave's step.
 constexpr int DEC_HEADS = 16;
 constexpr int DEC_WAVES = 4;
 constexpr int DEC_WAVE_TOK = 32;
-constexpr int DEC_TILE = DEC_WAVES * DEC_WAVE_TOK;
+constexpr int DEC_MAX_WG = 1024;
 
 struct AppendArgs {
     const uint8_t *src[2];    // new keys, new values

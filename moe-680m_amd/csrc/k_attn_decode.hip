@@ -5,12 +5,16 @@
 // Bound by reading K and V once (4 bytes of K and V for 4 * group operations a head element, far
 // below the matrix rate), so all that matters is to keep every CU's loads in flight:
 //
-//   * Work is cut by the lengths as they are in device memory, not by the host's bound: a tile is
-//     DEC_TILE tokens of one (sequence, key-value head, 16 query heads), tiles are numbered
-//     through, and each of the n_wg resident workgroups takes an equal run of them.  A run that
-//     ends inside a sequence leaves a partial row (maximum, sum, unnormalised output); the last
-//     workgroup of a sequence to arrive joins its partials in their order (same bits every time).
-//   * A wave takes 32 tokens of a tile by itself, no barrier until the run leaves the sequence:
+//   * A unit is one (sequence, key-value head, up to 16 of its query heads).  Each wave of a
+//     workgroup takes 32 tokens of a unit at a step; `wpu` waves share a unit, so a workgroup has
+//     U = 4 / wpu units of one sequence at work (a group).  wpu = 4 splits a unit the widest;
+//     wpu = 1 leaves nothing to join between waves and has the longest runs.
+//   * Work is cut by the lengths as they are in device memory, not by the host's bound: the groups'
+//     steps are numbered through and each of the n_wg resident workgroups takes an equal run of
+//     them.  A run that ends inside a group leaves partial rows (maximum, sum, unnormalised
+//     output).  They are joined inside the launch, in their order (same bits every time): of each
+//     16 consecutive workgroups the last one to arrive joins theirs, of those the last one all.
+//   * A wave works by itself, no barrier until the run leaves the group:
 //       S^T[token][head] = K Q^T       16x16x32 products, A rows = tokens straight from memory
 //                                      (a lane's 16 bytes = 8 elements of one token)
 //       O^T[d][head] += V^T P^T        B = P^T is S^T's own register layout: lane (head, g) holds
@@ -27,10 +31,14 @@ namespace moe {
 
 namespace {
 
-// Tiles of a sequence: one at least, so that an empty one's row is written too.
-__device__ __forceinline__ int seq_tiles(const AttnArgs &a, int b, int cap) {
+constexpr int JOIN = 16; // workgroups whose partial rows one workgroup joins
+constexpr int JOIN_MAX = 64; // pieces of one join: JOIN, or the groups of JOIN of a launch
+static_assert(DEC_MAX_WG <= JOIN * JOIN_MAX, "two levels join all");
+
+// Steps of a sequence's group: one at least, so that an empty one's rows are written too.
+__device__ __forceinline__ int seq_steps(const AttnArgs &a, int b, int cap, int shift) {
     const int n = min(max(a.kv_len[b], 0), cap);
-    return max(1, (n + DEC_TILE - 1) / DEC_TILE);
+    return max(1, (n + (1 << shift) - 1) >> shift);
 }
 
 template <typename T, int D>
@@ -41,22 +49,29 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
     constexpr int VW = D >= 128 ? 8 : 4;     // elements of a lane's V load
     constexpr int VS = D / (16 * VW);        // loads a token
     typedef uint32_t vload __attribute__((ext_vector_type(VW / 2)));
+    // the waves' rows; in a join the pieces' maxima and sums, then their factors
     __shared__ float s_o[DEC_WAVES][DEC_HEADS][D];
     __shared__ float s_ml[DEC_WAVES][DEC_HEADS][2];
     __shared__ uint32_t s_scan[DEC_WAVES], s_find[2];
     __shared__ uint32_t s_last;
+    static_assert(sizeof s_o >= JOIN_MAX * DEC_WAVES * DEC_HEADS * 4, "a join's factors");
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int cap = a.max_pages << a.page_shift;
-    const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS, hb_n = a.hkv * gb;
+    const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS; // head blocks of a key-value head
+    const int wpu = 1 << a.wpu_shift, U = DEC_WAVES >> a.wpu_shift;
+    const int shift = 5 + a.wpu_shift;                    // log2 of a step's tokens
+    const int ng = a.hkv * gb / U;                        // groups of a sequence
+    const int sub = wave >> a.wpu_shift, wsub = wave & (wpu - 1);
+    const int rows = min(DEC_HEADS, a.group);             // row places of a unit
 
-    // ---- this workgroup's run of tiles [lo, hi): prefix sums over the sequences
+    // ---- this workgroup's run of steps [lo, hi): prefix sums over the sequences
     const int per = (a.n_seqs + 255) / 256;
     uint32_t mine = 0;
     for (int i = 0; i < per; ++i) {
         const int b = tid * per + i;
-        if (b < a.n_seqs) mine += (uint32_t)seq_tiles(a, b, cap);
+        if (b < a.n_seqs) mine += (uint32_t)seq_steps(a, b, cap, shift);
     }
     uint32_t incl = mine;
     for (int o = 1; o < 64; o <<= 1) {
@@ -71,19 +86,19 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
         total_seq += s_scan[w];
     }
     before += incl - mine;
-    const uint64_t total = (uint64_t)total_seq * hb_n;
+    const uint64_t total = (uint64_t)total_seq * ng;
     const uint32_t share = (uint32_t)((total + gridDim.x - 1) / gridDim.x);
     const uint64_t lo = (uint64_t)blockIdx.x * share;
     if (lo >= total) return;
     const uint64_t hi = lo + share < total ? lo + share : total;
     {
-        const uint64_t first = (uint64_t)before * hb_n;
-        if (first <= lo && lo < first + (uint64_t)mine * hb_n) {
+        const uint64_t first = (uint64_t)before * ng;
+        if (first <= lo && lo < first + (uint64_t)mine * ng) {
             uint32_t p = before;
             int b = tid * per;
             for (;; ++b) {
-                const uint32_t n = (uint32_t)seq_tiles(a, b, cap);
-                if (lo < (uint64_t)(p + n) * hb_n) break;
+                const uint32_t n = (uint32_t)seq_steps(a, b, cap, shift);
+                if (lo < (uint64_t)(p + n) * ng) break;
                 p += n;
             }
             s_find[0] = (uint32_t)b;
@@ -92,10 +107,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
     }
     __syncthreads();
     int b = uniform((int)s_find[0]);
-    uint64_t at = (uint64_t)(uint32_t)uniform((int)s_find[1]) * hb_n; // first tile of sequence b
-    int nt = uniform(seq_tiles(a, b, cap));
-    int hb = (int)((lo - at) / (uint32_t)nt);
-    uint64_t unit = at + (uint64_t)hb * nt; // first tile of (b, hb)
+    const uint64_t at = (uint64_t)(uint32_t)uniform((int)s_find[1]) * ng; // first step of sequence b
+    int nt = uniform(seq_steps(a, b, cap, shift));
+    int sg = (int)((lo - at) / (uint32_t)nt);
+    uint64_t unit = at + (uint64_t)sg * nt; // first step of group (b, sg)
 
     for (uint64_t pos = lo; pos < hi;) {
         const int t0 = (int)(pos - unit);
@@ -103,9 +118,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
         const int len = ldc(a.kv_len + b);
         const int seen = min(max(len, 0), cap);
         if (seen != len && tid == 0) raise(a.flags, MOE_DEVFLAG_BAD_SEQ);
-        const int hk = hb / gb, h0 = hk * a.group + (hb - hk * gb) * DEC_HEADS;
-        const int nh = min(DEC_HEADS, (hk + 1) * a.group - h0); // heads of this unit
-        const T *q = (const T *)a.q + b * a.q_stride + (int64_t)(h0 + min(c, nh - 1)) * D;
+        // a unit's key-value head, first query head and heads
+        auto head0 = [&](int hb) { return hb / gb * a.group + hb % gb * DEC_HEADS; };
+        auto heads = [&](int hb) { return min(DEC_HEADS, a.group - hb % gb * DEC_HEADS); };
+        const int hb = sg * U + sub, hk = hb / gb;
+        const T *q = (const T *)a.q + b * a.q_stride + (int64_t)(head0(hb) + min(c, heads(hb) - 1)) * D;
         x8 qf[KS];
 #pragma unroll
         for (int k = 0; k < KS; ++k) qf[k] = ldg<x8>(q + k * 32 + g * 8);
@@ -118,7 +135,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
         const uint8_t *kb = a.k + 2 * hk * a.head_stride, *vb = a.v + 2 * hk * a.head_stride;
         const int ts2 = (int)(2 * a.token_stride);
         const int mask = (1 << a.page_shift) - 1;
-        const int end = min(seen, t1 * DEC_TILE); // of this piece
+        const int end = min(seen, t1 << shift); // of this piece
         bool bad = false;
 
         // the two 16-token halves of a step: byte offset of the first token, tokens there
@@ -157,13 +174,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
                 for (int s = 0; s < VS; ++s) vf[j][s] = ldg<vload>(p + s * (32 * VW));
             }
         };
-        int tok = t0 * DEC_TILE + wave * DEC_WAVE_TOK;
+        int tok = (t0 << shift) + wsub * DEC_WAVE_TOK;
+        const int step = 1 << shift;
         if (tok < end) {
             place(tok);
             load_k();
             load_v(off, have);
         }
-        for (; tok < end; tok += DEC_TILE) {
+        for (; tok < end; tok += step) {
             const int hv[2] = {have[0], have[1]};
             f32x4 st[2];
 #pragma unroll
@@ -172,10 +190,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
 #pragma unroll
                 for (int k = 0; k < KS; ++k) st[i] = E::mfma16(kf[i][k], qf[k], st[i]);
             }
-            const bool more = tok + DEC_TILE < end;
+            const bool more = tok + step < end;
             int64_t nx_off[2] = {off[0], off[1]};
             if (more) {
-                place(tok + DEC_TILE);
+                place(tok + step);
                 load_k();
                 nx_off[0] = off[0];
                 nx_off[1] = off[1];
@@ -244,80 +262,123 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
                         f32x4{acc[s * VW + j][r], acc[s * VW + j + 1][r], acc[s * VW + j + 2][r], acc[s * VW + j + 3][r]};
         __syncthreads();
         const bool whole = t0 == 0 && t1 == nt;
-        const uint32_t slot = 2 * blockIdx.x + (t0 == 0 ? 1u : 0u);
-        constexpr int PER = DEC_HEADS * D / 256; // elements a thread: one head's, consecutive
-        const int hh = tid * PER / D, d0 = tid * PER % D;
-        float M = -INFINITY, f[DEC_WAVES], L = 0.f, x[PER];
-#pragma unroll
-        for (int w = 0; w < DEC_WAVES; ++w) M = fmaxf(M, s_ml[w][hh][0]);
-#pragma unroll
-        for (int w = 0; w < DEC_WAVES; ++w) {
-            f[w] = exp2_(s_ml[w][hh][0] - base_of(M));
-            L += f[w] * s_ml[w][hh][1];
-        }
-#pragma unroll
-        for (int i = 0; i < PER; ++i) x[i] = 0.f;
-#pragma unroll
-        for (int w = 0; w < DEC_WAVES; ++w)
-#pragma unroll
-            for (int i = 0; i < PER; ++i) x[i] += f[w] * s_o[w][hh][d0 + i];
-        bool write = whole;
-        if (!whole) {
-            if (hh < nh) {
-                float *po = a.part + ((size_t)slot * DEC_HEADS + hh) * D + d0;
-#pragma unroll
-                for (int i = 0; i < PER; i += 4) *(f32x4 *)(po + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
-                if (d0 == 0) *(f32x2 *)(a.part_ml + ((size_t)slot * DEC_HEADS + hh) * 2) = f32x2{M, L};
+        // Partial rows: slot 0 of a workgroup holds the piece of a group that began before it, slot 1
+        // that of one which goes on behind it.
+        const size_t prow = DEC_WAVES * DEC_HEADS; // rows of a slot
+        const size_t slot = 2 * (size_t)blockIdx.x + (t0 == 0 ? 1 : 0);
+        const int items = U * rows * (D / 4);
+        auto put = [&](int u, int hh, int d, f32x4 x, float M, float L) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            if (L == 0.f) x = f32x4{0.f, 0.f, 0.f, 0.f};
+            const int h = head0(sg * U + u) + hh;
+            *(u32x2 *)((T *)a.o + b * a.o_stride + (int64_t)h * D + d) =
+                u32x2{E::pack(x[0] * inv, x[1] * inv), E::pack(x[2] * inv, x[3] * inv)};
+            if (a.lse && d == 0)
+                a.lse[(int64_t)b * a.hq + h] =
+                    L == 0.f ? -INFINITY : (base_of(M) - E::SHIFT + __log2f(L)) * 0.69314718055994531f;
+        };
+        for (int i = tid; i < items; i += 256) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4, u = r / rows, hh = r % rows;
+            if (hh >= heads(sg * U + u)) continue;
+            const int w0 = u << a.wpu_shift;
+            float M = -INFINITY, L = 0.f;
+            for (int w = 0; w < wpu; ++w) M = fmaxf(M, s_ml[w0 + w][hh][0]);
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+            for (int w = 0; w < wpu; ++w) {
+                const float f = exp2_(s_ml[w0 + w][hh][0] - base_of(M));
+                L += f * s_ml[w0 + w][hh][1];
+                x += f * *(const f32x4 *)&s_o[w0 + w][hh][d];
             }
-            // the pieces of this unit: workgroups w0 (its tail slot) to w1 (their head slots)
+            if (whole) put(u, hh, d, x, M, L);
+            else {
+                publish(a.part + (slot * prow + u * DEC_HEADS + hh) * D + d, x);
+                if (d == 0) publish(a.part_ml + (slot * prow + u * DEC_HEADS + hh) * 2, f32x2{M, L});
+            }
+        }
+        if (!whole) {
+            // the group's pieces: workgroups w0 (slot 1) to w1 (slot 0)
             const uint32_t w0 = (uint32_t)(unit / share), w1 = (uint32_t)((unit + nt - 1) / share);
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) s_last = atomicAdd(a.arrived + w0, 1u);
-            __syncthreads();
-            if (s_last == w1 - w0) {
-                __threadfence();
-                write = true;
-                if (tid == 0) a.arrived[w0] = 0;
-                M = -INFINITY;
-                L = 0.f;
+            uint32_t wa = blockIdx.x / JOIN * JOIN;
+            const uint32_t wb = min(wa + JOIN - 1, w1);
+            wa = max(wa, w0);
+            uint32_t first = wa, stride = 1, n = wb - wa + 1;
+            uint32_t *count = a.arrived + 2 * wa + (wa == w0 ? 1 : 0);
+            for (int level = 0;; ++level) {
+                __syncthreads(); // waits for this piece's stores
+                if (tid == 0) {
+                    s_last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    if (s_last == n - 1) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                __syncthreads();
+                if (s_last != n - 1) break;
+                // piece p's slot: workgroup first + p stride, of w0 the later one, and of a joined
+                // group of JOIN its first workgroup's
+                auto at_piece = [&](uint32_t p) {
+                    uint32_t w = first + p * stride;
+                    if (level) w = p == 0 ? w0 : w / JOIN * JOIN;
+                    return 2 * (size_t)w + (w == w0 ? 1 : 0);
+                };
+                const int R = U * rows;
+                float *fac = &s_o[0][0][0];                     // [n][R]
+                f32x2 *ml = (f32x2 *)&s_ml[0][0][0];            // [R]: the joined maximum and sum
+                for (int r = tid; r < R; r += 256) {
+                    const int u = r / rows, hh = r % rows;
+                    const float *src = a.part_ml + (size_t)(u * DEC_HEADS + hh) * 2;
+                    float M = -INFINITY, L = 0.f;
+                    for (uint32_t p = 0; p < n; p += 8) {
+                        f32x2 v[8];
 #pragma unroll
-                for (int i = 0; i < PER; ++i) x[i] = 0.f;
-                if (hh < nh)
-                    for (uint32_t w = w0; w <= w1; ++w) {
-                        const size_t sl = ((size_t)(2 * w + (w == w0 ? 1u : 0u)) * DEC_HEADS + hh);
-                        const f32x2 ml = *(const f32x2 *)(a.part_ml + sl * 2);
-                        const float mx = fmaxf(M, ml.x), fo = exp2_(M - base_of(mx)), fn = exp2_(ml.x - base_of(mx));
+                        for (int j = 0; j < 8; ++j)
+                            v[j] = p + j < n ? remote2(src + at_piece(p + j) * prow * 2) : f32x2{-INFINITY, 0.f};
+                        float mx = M;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) mx = fmaxf(mx, v[j].x);
+                        L *= exp2_(M - base_of(mx));
                         M = mx;
-                        L = L * fo + ml.y * fn;
-                        const float *po = a.part + sl * D + d0;
 #pragma unroll
-                        for (int i = 0; i < PER; i += 4) {
-                            const f32x4 v = *(const f32x4 *)(po + i);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) x[i + j] = x[i + j] * fo + v[j] * fn;
+                        for (int j = 0; j < 8; ++j) {
+                            L += v[j].y * exp2_(v[j].x - base_of(M));
+                            if (p + j < n) fac[(p + j) * R + r] = v[j].x;
                         }
                     }
-            }
-        }
-        if (write && hh < nh) {
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            T *o = (T *)a.o + b * a.o_stride + (int64_t)(h0 + hh) * D + d0;
+                    for (uint32_t p = 0; p < n; ++p) fac[p * R + r] = exp2_(fac[p * R + r] - base_of(M));
+                    ml[r] = f32x2{M, L};
+                }
+                __syncthreads();
+                const bool final = level || w0 / JOIN == w1 / JOIN;
+                for (int i = tid; i < items; i += 256) {
+                    const int r = i / (D / 4), d = i % (D / 4) * 4, u = r / rows, hh = r % rows;
+                    if (hh >= heads(sg * U + u)) continue;
+                    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                    const float *src = a.part + (size_t)(u * DEC_HEADS + hh) * D + d;
+                    for (uint32_t p = 0; p < n; p += 8) {
+                        f32x4 v[8];
 #pragma unroll
-            for (int i = 0; i < PER; i += 2)
-                *(uint32_t *)(o + i) = E::pack(L == 0.f ? 0.f : x[i] * inv, L == 0.f ? 0.f : x[i + 1] * inv);
-            if (a.lse && d0 == 0)
-                a.lse[(int64_t)b * a.hq + h0 + hh] =
-                    L == 0.f ? -INFINITY : (base_of(M) - E::SHIFT + __log2f(L)) * 0.69314718055994531f;
+                        for (int j = 0; j < 8; ++j)
+                            v[j] = p + j < n ? remote4(src + at_piece(p + j) * prow * D) : f32x4{};
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) x += (p + j < n ? fac[(p + j) * R + r] : 0.f) * v[j];
+                    }
+                    if (final) put(u, hh, d, x, ml[r].x, ml[r].y);
+                    else publish(a.part + (at_piece(0) * prow + u * DEC_HEADS + hh) * D + d, x);
+                }
+                if (final) break;
+                for (int r = tid; r < R; r += 256)
+                    publish(a.part_ml + (at_piece(0) * prow + r / rows * DEC_HEADS + r % rows) * 2, ml[r]);
+                first = w0 / JOIN * JOIN;
+                stride = JOIN;
+                n = w1 / JOIN - w0 / JOIN + 1;
+                count = a.arrived + 2 * gridDim.x + w0;
+            }
         }
         pos = unit + t1;
         if (pos < hi) { // the next (sequence, heads)
             __syncthreads(); // s_o is free again
             unit += nt;
-            if (++hb == hb_n) {
-                hb = 0;
+            if (++sg == ng) {
+                sg = 0;
                 ++b;
-                nt = uniform(seq_tiles(a, b, cap));
+                nt = uniform(seq_steps(a, b, cap, shift));
             }
         }
     }
@@ -334,7 +395,14 @@ hipError_t decode_d(const AttnArgs &a, int d, hipStream_t st) {
 
 } // namespace
 
-hipError_t launch_attn_decode(const AttnArgs &a, int type, int d, hipStream_t st) {
+hipError_t launch_attn_decode(const AttnArgs &args, int type, int d, hipStream_t st) {
+    AttnArgs a = args;
+    // Units enough for every workgroup to have several at once: let fewer waves share one.
+    const int hb = a.hkv * ((a.group + DEC_HEADS - 1) / DEC_HEADS);
+    const int64_t units = (int64_t)a.n_seqs * hb;
+    a.wpu_shift = 2;
+    if (hb % 4 == 0 && units >= 4 * a.n_wg) a.wpu_shift = 0;
+    else if (hb % 2 == 0 && units >= 2 * a.n_wg) a.wpu_shift = 1;
     return type == MOE_T_F16 ? decode_d<f16_t>(a, d, st) : decode_d<bf16_t>(a, d, st);
 }
 
