@@ -63,6 +63,12 @@ __device__ __forceinline__ T ldc(const T *p) {
     return *(const __attribute__((address_space(4))) T *)p;
 }
 
+// A load at a lane's 32-bit offset from an address that is the same in all lanes.
+template <typename T>
+__device__ __forceinline__ T ldo(const uint8_t *base, uint32_t off) {
+    return *(const MOE_GLOBAL T *)((const MOE_GLOBAL uint8_t *)base + off);
+}
+
 // Partial rows that workgroups on other XCDs (each with an L2 of its own) join: stored at agent scope,
 // which writes through the producer's L2, and read at system scope, past the reader's.  A
 // workgroup's barrier waits for its stores, so a count added behind the barrier says that they are

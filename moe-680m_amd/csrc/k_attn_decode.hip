@@ -123,9 +123,15 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
         auto heads = [&](int hb) { return min(DEC_HEADS, a.group - hb % gb * DEC_HEADS); };
         const int hb = sg * U + sub, hk = hb / gb;
         const T *q = (const T *)a.q + b * a.q_stride + (int64_t)(head0(hb) + min(c, heads(hb) - 1)) * D;
+        // The queries' fragments stay in registers; at D = 256, where those are short, in the wave's own
+        // part of s_o, every lane reading back what it wrote.
         x8 qf[KS];
+        x8 *const ql = (x8 *)&s_o[wave][0][0] + lane;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) qf[k] = ldg<x8>(q + k * 32 + g * 8);
+        for (int k = 0; k < KS; ++k) {
+            qf[k] = ldg<x8>(q + k * 32 + g * 8);
+            if (D == 256) ql[64 * k] = qf[k];
+        }
 
         f32x4 acc[D / 16];
 #pragma unroll
@@ -157,21 +163,25 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
         x8 kf[2][KS];
         vload vf[8][VS];
         // a lane whose token is not there reads the last one that is (the first place if none is)
+        auto lane_off = [&](int t, int i, int byte) {
+            if (have[i] < 16) t = max(0, min(t, have[i] - 1));
+            return (uint32_t)(t * ts2 + byte);
+        };
         auto load_k = [&]() {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const uint8_t *p = kb + off[i] + max(0, min(c, have[i] - 1)) * ts2 + g * 16;
+                const uint32_t lo = lane_off(c, i, g * 16);
 #pragma unroll
-                for (int k = 0; k < KS; ++k) kf[i][k] = ldg<x8>(p + k * 64);
+                for (int k = 0; k < KS; ++k) kf[i][k] = ldo<x8>(kb + off[i], lo + k * 64);
             }
         };
-        auto load_v = [&](const int64_t *off, const int *have) {
+        auto load_v = [&]() {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int i = j >> 2, t = max(0, min(4 * g + (j & 3), have[i] - 1));
-                const uint8_t *p = vb + off[i] + t * ts2 + c * (VW * 2);
+                const int i = j >> 2;
+                const uint32_t lo = lane_off(4 * g + (j & 3), i, c * (VW * 2));
 #pragma unroll
-                for (int s = 0; s < VS; ++s) vf[j][s] = ldg<vload>(p + s * (32 * VW));
+                for (int s = 0; s < VS; ++s) vf[j][s] = ldo<vload>(vb + off[i], lo + s * (32 * VW));
             }
         };
         int tok = (t0 << shift) + wsub * DEC_WAVE_TOK;
@@ -179,24 +189,23 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
         if (tok < end) {
             place(tok);
             load_k();
-            load_v(off, have);
+            load_v();
         }
         for (; tok < end; tok += step) {
             const int hv[2] = {have[0], have[1]};
             f32x4 st[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                st[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < KS; ++k) {
+                const x8 qk = D == 256 ? ql[64 * k] : qf[k];
+                if (D == 256 && k % 2 == 0) __builtin_amdgcn_sched_barrier(0); // not all of them at once
 #pragma unroll
-                for (int k = 0; k < KS; ++k) st[i] = E::mfma16(kf[i][k], qf[k], st[i]);
+                for (int i = 0; i < 2; ++i)
+                    st[i] = E::mfma16(kf[i][k], qk, k ? st[i] : f32x4{0.f, 0.f, 0.f, 0.f});
             }
             const bool more = tok + step < end;
-            int64_t nx_off[2] = {off[0], off[1]};
             if (more) {
                 place(tok + step);
                 load_k();
-                nx_off[0] = off[0];
-                nx_off[1] = off[1];
             }
             float mx = m;
 #pragma unroll
@@ -240,7 +249,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
                     a0 = E::mfma16(__builtin_bit_cast(x8, e0), pf, a0);
                     a1 = E::mfma16(__builtin_bit_cast(x8, e1), pf, a1);
                 }
-            if (more) load_v(nx_off, have);
+            if (more) load_v();
         }
         if (bad && lane == 0) raise(a.flags, MOE_DEVFLAG_BAD_PAGE);
 
