@@ -17,7 +17,7 @@ struct moe_attn {
     uint32_t *flags = nullptr; // sticky device flags
     float *part = nullptr;     // decode partials: [2 n_wg][DEC_WAVES][DEC_HEADS][head_dim]
     float *part_ml = nullptr;  // [2 n_wg][DEC_WAVES][DEC_HEADS][2]
-    uint32_t *arrived = nullptr; // [3 n_wg], zero between calls
+    Piece *piece = nullptr;    // [n_wg]
     int n_wg = 0;              // workgroups of a decode launch
 };
 
@@ -71,6 +71,11 @@ moe_status common_args(const char *fn, moe_attn *a, const moe_kv_cache *kv, cons
         if (v < g.head_dim || (v & 7) || v > ((int64_t)1 << 40) || kv->token_stride > (1 << 24))
             return fail(MOE_EINVAL, "%s: cache stride %lld (multiples of 8, head_dim=%d at least; token_stride at most 2^24)", fn,
                         (long long)v, g.head_dim);
+    // steps of 32 tokens, of every sequence and head, are counted in 32 bits
+    const int64_t blocks = (int64_t)g.n_kv_heads * ((g.n_q_heads / g.n_kv_heads + DEC_HEADS - 1) / DEC_HEADS);
+    if ((((int64_t)s->max_pages << a->page_shift) / 32 + 1) * s->n_seqs * blocks >= ((int64_t)1 << 31))
+        return fail(MOE_EINVAL, "%s: %d page lists of %d pages of %d tokens are too long together", fn, s->n_seqs,
+                    s->max_pages, g.page_tokens);
     *c = AttnArgs{};
     if (s->n_seqs == 0 || s->n_rows == 0) return MOE_OK; // nothing to do: no other pointer is needed
     if (!kv->k || !kv->v || !s->pages || !s->kv_len) return fail(MOE_EINVAL, "%s: null argument", fn);
@@ -121,7 +126,7 @@ moe_status attn_call(const char *fn, moe_attn *a, const moe_kv_cache *kv, const 
     c.scale_log2 = (float)(scale * 1.4426950408889634);
     c.part = a->part;
     c.part_ml = a->part_ml;
-    c.arrived = a->arrived;
+    c.piece = a->piece;
     c.n_wg = a->n_wg;
     OnDevice on(a->device);
     hipError_t he = on.he;
@@ -170,7 +175,7 @@ moe_status moe_attn_create(int device, const moe_attn_config *cfg, moe_attn **ou
         size_t bytes;
     } parts[] = {
         {(void **)&a->flags, 256},
-        {(void **)&a->arrived, (size_t)a->n_wg * 3 * 4},
+        {(void **)&a->piece, (size_t)a->n_wg * sizeof(Piece)},
         {(void **)&a->part_ml, (size_t)a->n_wg * 2 * DEC_WAVES * DEC_HEADS * 2 * 4},
         {(void **)&a->part, (size_t)a->n_wg * 2 * DEC_WAVES * DEC_HEADS * g.head_dim * 4},
     };

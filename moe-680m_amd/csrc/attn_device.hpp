@@ -63,32 +63,35 @@ __device__ __forceinline__ T ldc(const T *p) {
     return *(const __attribute__((address_space(4))) T *)p;
 }
 
-// A load at a lane's 32-bit offset from an address that is the same in all lanes.
+// A load at a lane's 32-bit offset (and a constant) from an address that is the same in all lanes.
 template <typename T>
-__device__ __forceinline__ T ldo(const uint8_t *base, uint32_t off) {
-    return *(const MOE_GLOBAL T *)((const MOE_GLOBAL uint8_t *)base + off);
+__device__ __forceinline__ T ldo(const uint8_t *base, uint32_t off, int imm = 0) {
+    return *(const MOE_GLOBAL T *)((const MOE_GLOBAL uint8_t *)base + off + imm);
 }
 
-// Partial rows that workgroups on other XCDs (each with an L2 of its own) join: stored at agent scope,
-// which writes through the producer's L2, and read at system scope, past the reader's.  A
-// workgroup's barrier waits for its stores, so a count added behind the barrier says that they are
-// there.  Fences in their place write back and invalidate whole L2s: 10 us and more a join.
-__device__ __forceinline__ void publish(float *p, f32x2 v) {
-    __hip_atomic_store((MOE_GLOBAL uint64_t *)p, __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED,
-                       __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void publish(float *p, f32x4 v) {
-    publish(p, f32x2{v[0], v[1]});
-    publish(p + 2, f32x2{v[2], v[3]});
-}
-__device__ __forceinline__ f32x4 remote4(const float *p) {
-    return __builtin_bit_cast(f32x4, remote_quad((const u32x4 *)p));
-}
-__device__ __forceinline__ f32x2 remote2(const float *p) {
-    return __builtin_bit_cast(f32x2, __hip_atomic_load((const MOE_GLOBAL uint64_t *)p, __ATOMIC_RELAXED,
-                                                       __HIP_MEMORY_SCOPE_SYSTEM));
+// The kernel's argument block (its only argument), read again: where only an epilogue uses them, the
+// arguments are not held in scalar registers through the loop before it.
+__device__ __forceinline__ const __attribute__((address_space(4))) AttnArgs &fresh_args() {
+    auto p = (const __attribute__((address_space(4))) AttnArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *p;
 }
 
+// Inclusive sum over the wave's lanes.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false); // row_shr:1
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, false); // row_shr:2
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, false); // row_shr:4
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, false); // row_shr:8
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false); // row_bcast:15
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false); // row_bcast:31
+    return x;
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+    for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+    return x;
+}
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 } // namespace moe

@@ -8,6 +8,12 @@
 
 namespace moe {
 
+// A group of rows that several workgroups computed a piece of: rows of sequence b, head group sg, the
+// pieces n of workgroups w0 and on (n < 2: nothing to join).
+struct Piece {
+    int b, sg, w0, n;
+};
+
 // One call's sequences, cache and rows (see moe_seq_batch and moe_kv_cache for the layout).
 struct AttnArgs {
     const void *q;
@@ -26,7 +32,7 @@ struct AttnArgs {
     float scale_log2;         // scale * log2(e): exponentials are taken in base 2
     float *part;              // workspace: partial rows of pieces (see k_attn_decode.hip)
     float *part_ml;           // ... and each partial row's running maximum and sum
-    uint32_t *arrived;        // ... and counts of the pieces that have arrived (zero between calls)
+    Piece *piece;             // ... and the groups to join
     int n_wg;                 // workgroups of a decode launch
     int wpu_shift;            // decode: log2 of the waves that share a unit
 };

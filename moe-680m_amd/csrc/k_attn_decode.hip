@@ -12,8 +12,7 @@
 //   * Work is cut by the lengths as they are in device memory, not by the host's bound: the groups'
 //     steps are numbered through and each of the n_wg resident workgroups takes an equal run of
 //     them.  A run that ends inside a group leaves partial rows (maximum, sum, unnormalised
-//     output).  They are joined inside the launch, in their order (same bits every time): of each
-//     16 consecutive workgroups the last one to arrive joins theirs, of those the last one all.
+//     output), which a second launch joins in their order (same bits every time).
 //   * A wave works by itself, no barrier until the run leaves the group:
 //       S^T[token][head] = K Q^T       16x16x32 products, A rows = tokens straight from memory
 //                                      (a lane's 16 bytes = 8 elements of one token)
@@ -31,14 +30,29 @@ namespace moe {
 
 namespace {
 
-constexpr int JOIN = 16; // workgroups whose partial rows one workgroup joins
-constexpr int JOIN_MAX = 64; // pieces of one join: JOIN, or the groups of JOIN of a launch
-static_assert(DEC_MAX_WG <= JOIN * JOIN_MAX, "two levels join all");
-
 // Steps of a sequence's group: one at least, so that an empty one's rows are written too.
 __device__ __forceinline__ int seq_steps(const AttnArgs &a, int b, int cap, int shift) {
     const int n = min(max(a.kv_len[b], 0), cap);
     return max(1, (n + (1 << shift) - 1) >> shift);
+}
+
+// A partial row's maximum and sum: those of a row place lie together, so that a wave loads many
+// pieces' at once.
+template <typename Args>
+__device__ __forceinline__ size_t ml_at(const Args &a, int place, size_t slot) {
+    return (size_t)place * (4 * a.n_wg) + 2 * slot;
+}
+
+// Four elements of a finished row: x / L, and with the first ones the log of the sum.
+template <typename T, typename Args>
+__device__ __forceinline__ void put_row(const Args &a, int b, int h, int D, int d, f32x4 x, float M, float L) {
+    typedef Elem<T> E;
+    const float inv = 1.f / L;
+    x = L == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : x * inv;
+    *(u32x2 *)((T *)a.o + b * a.o_stride + (int64_t)h * D + d) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+    if (a.lse && d == 0)
+        a.lse[(int64_t)b * a.hq + h] =
+            L == 0.f ? -INFINITY : (base_of(M) - E::SHIFT + __log2f(L)) * 0.69314718055994531f;
 }
 
 template <typename T, int D>
@@ -49,12 +63,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
     constexpr int VW = D >= 128 ? 8 : 4;     // elements of a lane's V load
     constexpr int VS = D / (16 * VW);        // loads a token
     typedef uint32_t vload __attribute__((ext_vector_type(VW / 2)));
-    // the waves' rows; in a join the pieces' maxima and sums, then their factors
-    __shared__ float s_o[DEC_WAVES][DEC_HEADS][D];
-    __shared__ float s_ml[DEC_WAVES][DEC_HEADS][2];
-    __shared__ uint32_t s_scan[DEC_WAVES], s_find[2];
-    __shared__ uint32_t s_last;
-    static_assert(sizeof s_o >= JOIN_MAX * DEC_WAVES * DEC_HEADS * 4, "a join's factors");
+    // the waves' rows, 4 floats apart so that 16 lanes' rows start in different banks
+    constexpr int OS = D + 4;
+    constexpr int ROWS = DEC_WAVES * DEC_HEADS; // row places of a group
+    __shared__ float s_o[DEC_WAVES][DEC_HEADS][OS];
+    __shared__ f32x2 s_ml[DEC_WAVES][DEC_HEADS];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
@@ -66,72 +79,55 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
     const int sub = wave >> a.wpu_shift, wsub = wave & (wpu - 1);
     const int rows = min(DEC_HEADS, a.group);             // row places of a unit
 
-    // ---- this workgroup's run of steps [lo, hi): prefix sums over the sequences
-    const int per = (a.n_seqs + 255) / 256;
+    // ---- this workgroup's run of steps [lo, hi): every wave sums the sequences' steps by itself,
+    // a lane those of `per` in a row, and finds the sequence that lo lies in
+    const int per = (a.n_seqs + 63) / 64;
     uint32_t mine = 0;
     for (int i = 0; i < per; ++i) {
-        const int b = tid * per + i;
+        const int b = lane * per + i;
         if (b < a.n_seqs) mine += (uint32_t)seq_steps(a, b, cap, shift);
     }
-    uint32_t incl = mine;
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t v = __shfl_up(incl, o);
-        if (lane >= o) incl += v;
+    const uint32_t incl = wave_scan(mine);
+    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63) * ng;
+    const uint32_t share = (total + gridDim.x - 1) / gridDim.x;
+    const uint32_t lo = blockIdx.x * share;
+    if (lo >= total) {
+        if (tid == 0 && (int64_t)a.n_seqs * ng > a.n_wg) a.piece[blockIdx.x] = Piece{0, 0, 0, 0};
+        return;
     }
-    if (lane == 63) s_scan[wave] = incl;
-    __syncthreads();
-    uint32_t before = 0, total_seq = 0;
-    for (int w = 0; w < DEC_WAVES; ++w) {
-        if (w < wave) before += s_scan[w];
-        total_seq += s_scan[w];
+    const uint32_t hi = min(lo + share, total);
+    const int owner = __builtin_ctzll(__ballot(incl * ng > lo));
+    uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), owner); // steps before b, of one group
+    int b = owner * per, nt = uniform(seq_steps(a, b, cap, shift));
+    while ((at + nt) * ng <= lo) {
+        at += nt;
+        nt = uniform(seq_steps(a, ++b, cap, shift));
     }
-    before += incl - mine;
-    const uint64_t total = (uint64_t)total_seq * ng;
-    const uint32_t share = (uint32_t)((total + gridDim.x - 1) / gridDim.x);
-    const uint64_t lo = (uint64_t)blockIdx.x * share;
-    if (lo >= total) return;
-    const uint64_t hi = lo + share < total ? lo + share : total;
-    {
-        const uint64_t first = (uint64_t)before * ng;
-        if (first <= lo && lo < first + (uint64_t)mine * ng) {
-            uint32_t p = before;
-            int b = tid * per;
-            for (;; ++b) {
-                const uint32_t n = (uint32_t)seq_steps(a, b, cap, shift);
-                if (lo < (uint64_t)(p + n) * ng) break;
-                p += n;
-            }
-            s_find[0] = (uint32_t)b;
-            s_find[1] = p;
-        }
-    }
-    __syncthreads();
-    int b = uniform((int)s_find[0]);
-    const uint64_t at = (uint64_t)(uint32_t)uniform((int)s_find[1]) * ng; // first step of sequence b
-    int nt = uniform(seq_steps(a, b, cap, shift));
-    int sg = (int)((lo - at) / (uint32_t)nt);
-    uint64_t unit = at + (uint64_t)sg * nt; // first step of group (b, sg)
+    int sg = (int)((lo - at * ng) / (uint32_t)nt);
+    uint32_t unit = at * ng + sg * nt; // first step of group (b, sg)
 
-    for (uint64_t pos = lo; pos < hi;) {
+    // a unit's key-value head, first query head and heads
+    auto head0 = [&](int hb) { return hb / gb * a.group + hb % gb * DEC_HEADS; };
+    auto heads = [&](int hb) { return min(DEC_HEADS, a.group - hb % gb * DEC_HEADS); };
+    const int items = U * rows * (D / 4);
+    // For the join: of every group the pieces it was cut into, or (more groups than workgroups) of every
+    // workgroup those of the group that it begins and others go on with.
+    const bool by_group = (int64_t)a.n_seqs * ng <= a.n_wg;
+    Piece tail = {0, 0, 0, 0};
+
+    for (uint32_t pos = lo; pos < hi;) {
         const int t0 = (int)(pos - unit);
         const int t1 = (int)((hi < unit + nt ? hi : unit + nt) - unit);
         const int len = ldc(a.kv_len + b);
         const int seen = min(max(len, 0), cap);
         if (seen != len && tid == 0) raise(a.flags, MOE_DEVFLAG_BAD_SEQ);
-        // a unit's key-value head, first query head and heads
-        auto head0 = [&](int hb) { return hb / gb * a.group + hb % gb * DEC_HEADS; };
-        auto heads = [&](int hb) { return min(DEC_HEADS, a.group - hb % gb * DEC_HEADS); };
         const int hb = sg * U + sub, hk = hb / gb;
         const T *q = (const T *)a.q + b * a.q_stride + (int64_t)(head0(hb) + min(c, heads(hb) - 1)) * D;
         // The queries' fragments stay in registers; at D = 256, where those are short, in the wave's own
         // part of s_o, every lane reading back what it wrote.
         x8 qf[KS];
-        x8 *const ql = (x8 *)&s_o[wave][0][0] + lane;
 #pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            qf[k] = ldg<x8>(q + k * 32 + g * 8);
-            if (D == 256) ql[64 * k] = qf[k];
-        }
+        for (int k = 0; k < KS; ++k) qf[k] = ldg<x8>(q + k * 32 + g * 8);
 
         f32x4 acc[D / 16];
 #pragma unroll
@@ -172,7 +168,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
             for (int i = 0; i < 2; ++i) {
                 const uint32_t lo = lane_off(c, i, g * 16);
 #pragma unroll
-                for (int k = 0; k < KS; ++k) kf[i][k] = ldo<x8>(kb + off[i], lo + k * 64);
+                for (int k = 0; k < KS; ++k) kf[i][k] = ldo<x8>(kb + off[i], lo, k * 64);
             }
         };
         auto load_v = [&]() {
@@ -181,7 +177,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
                 const int i = j >> 2;
                 const uint32_t lo = lane_off(4 * g + (j & 3), i, c * (VW * 2));
 #pragma unroll
-                for (int s = 0; s < VS; ++s) vf[j][s] = ldo<vload>(vb + off[i], lo + s * (32 * VW));
+                for (int s = 0; s < VS; ++s) vf[j][s] = ldo<vload>(vb + off[i], lo, s * (32 * VW));
             }
         };
         int tok = (t0 << shift) + wsub * DEC_WAVE_TOK;
@@ -191,6 +187,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
             load_k();
             load_v();
         }
+        x8 *const ql = (x8 *)&s_o[wave][0][0] + lane;
+        if (D == 256)
+#pragma unroll
+            for (int k = 0; k < KS; ++k) ql[64 * k] = qf[k];
         for (; tok < end; tok += step) {
             const int hv[2] = {have[0], have[1]};
             f32x4 st[2];
@@ -256,10 +256,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
         // ---- join the four waves: row (head c) of O^T's register layout to s_o[wave][head][d]
         l += __shfl_xor(l, 16);
         l += __shfl_xor(l, 32);
-        if (g == 0) {
-            s_ml[wave][c][0] = m;
-            s_ml[wave][c][1] = l;
-        }
+        if (g == 0) s_ml[wave][c] = f32x2{m, l};
         // the row's elements 16 VW s + VW (4 g + r) + j, j = 0..VW-1
 #pragma unroll
         for (int s = 0; s < VS; ++s)
@@ -271,114 +268,44 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
                         f32x4{acc[s * VW + j][r], acc[s * VW + j + 1][r], acc[s * VW + j + 2][r], acc[s * VW + j + 3][r]};
         __syncthreads();
         const bool whole = t0 == 0 && t1 == nt;
+        int et = tid; // opaque, so that no item's index is computed before the loop and held through it
+        asm volatile("" : "+v"(et));
         // Partial rows: slot 0 of a workgroup holds the piece of a group that began before it, slot 1
         // that of one which goes on behind it.
-        const size_t prow = DEC_WAVES * DEC_HEADS; // rows of a slot
         const size_t slot = 2 * (size_t)blockIdx.x + (t0 == 0 ? 1 : 0);
-        const int items = U * rows * (D / 4);
-        auto put = [&](int u, int hh, int d, f32x4 x, float M, float L) {
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            if (L == 0.f) x = f32x4{0.f, 0.f, 0.f, 0.f};
-            const int h = head0(sg * U + u) + hh;
-            *(u32x2 *)((T *)a.o + b * a.o_stride + (int64_t)h * D + d) =
-                u32x2{E::pack(x[0] * inv, x[1] * inv), E::pack(x[2] * inv, x[3] * inv)};
-            if (a.lse && d == 0)
-                a.lse[(int64_t)b * a.hq + h] =
-                    L == 0.f ? -INFINITY : (base_of(M) - E::SHIFT + __log2f(L)) * 0.69314718055994531f;
-        };
-        for (int i = tid; i < items; i += 256) {
+        for (int i = et; i < items; i += 256) {
             const int r = i / (D / 4), d = i % (D / 4) * 4, u = r / rows, hh = r % rows;
             if (hh >= heads(sg * U + u)) continue;
             const int w0 = u << a.wpu_shift;
-            float M = -INFINITY, L = 0.f;
-            for (int w = 0; w < wpu; ++w) M = fmaxf(M, s_ml[w0 + w][hh][0]);
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
-            for (int w = 0; w < wpu; ++w) {
-                const float f = exp2_(s_ml[w0 + w][hh][0] - base_of(M));
-                L += f * s_ml[w0 + w][hh][1];
-                x += f * *(const f32x4 *)&s_o[w0 + w][hh][d];
+            f32x2 ml[DEC_WAVES];
+            f32x4 y[DEC_WAVES];
+#pragma unroll
+            for (int w = 0; w < DEC_WAVES; ++w) { // fewer waves: some twice, the second time as nothing
+                ml[w] = s_ml[w0 + (w & (wpu - 1))][hh];
+                y[w] = *(const f32x4 *)&s_o[w0 + (w & (wpu - 1))][hh][d];
             }
-            if (whole) put(u, hh, d, x, M, L);
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int w = 0; w < DEC_WAVES; ++w) M = fmaxf(M, ml[w].x);
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < DEC_WAVES; ++w)
+                if (w < wpu) {
+                    const float f = exp2_(ml[w].x - base_of(M));
+                    L += f * ml[w].y;
+                    x += f * y[w];
+                }
+            if (whole) put_row<T>(a, b, head0(sg * U + u) + hh, D, d, x, M, L);
             else {
-                publish(a.part + (slot * prow + u * DEC_HEADS + hh) * D + d, x);
-                if (d == 0) publish(a.part_ml + (slot * prow + u * DEC_HEADS + hh) * 2, f32x2{M, L});
+                *(f32x4 *)(a.part + (slot * ROWS + u * DEC_HEADS + hh) * D + d) = x;
+                if (d == 0) *(f32x2 *)(a.part_ml + ml_at(a, u * DEC_HEADS + hh, slot)) = f32x2{M, L};
             }
         }
-        if (!whole) {
-            // the group's pieces: workgroups w0 (slot 1) to w1 (slot 0)
-            const uint32_t w0 = (uint32_t)(unit / share), w1 = (uint32_t)((unit + nt - 1) / share);
-            uint32_t wa = blockIdx.x / JOIN * JOIN;
-            const uint32_t wb = min(wa + JOIN - 1, w1);
-            wa = max(wa, w0);
-            uint32_t first = wa, stride = 1, n = wb - wa + 1;
-            uint32_t *count = a.arrived + 2 * wa + (wa == w0 ? 1 : 0);
-            for (int level = 0;; ++level) {
-                __syncthreads(); // waits for this piece's stores
-                if (tid == 0) {
-                    s_last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    if (s_last == n - 1) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                }
-                __syncthreads();
-                if (s_last != n - 1) break;
-                // piece p's slot: workgroup first + p stride, of w0 the later one, and of a joined
-                // group of JOIN its first workgroup's
-                auto at_piece = [&](uint32_t p) {
-                    uint32_t w = first + p * stride;
-                    if (level) w = p == 0 ? w0 : w / JOIN * JOIN;
-                    return 2 * (size_t)w + (w == w0 ? 1 : 0);
-                };
-                const int R = U * rows;
-                float *fac = &s_o[0][0][0];                     // [n][R]
-                f32x2 *ml = (f32x2 *)&s_ml[0][0][0];            // [R]: the joined maximum and sum
-                for (int r = tid; r < R; r += 256) {
-                    const int u = r / rows, hh = r % rows;
-                    const float *src = a.part_ml + (size_t)(u * DEC_HEADS + hh) * 2;
-                    float M = -INFINITY, L = 0.f;
-                    for (uint32_t p = 0; p < n; p += 8) {
-                        f32x2 v[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            v[j] = p + j < n ? remote2(src + at_piece(p + j) * prow * 2) : f32x2{-INFINITY, 0.f};
-                        float mx = M;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) mx = fmaxf(mx, v[j].x);
-                        L *= exp2_(M - base_of(mx));
-                        M = mx;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            L += v[j].y * exp2_(v[j].x - base_of(M));
-                            if (p + j < n) fac[(p + j) * R + r] = v[j].x;
-                        }
-                    }
-                    for (uint32_t p = 0; p < n; ++p) fac[p * R + r] = exp2_(fac[p * R + r] - base_of(M));
-                    ml[r] = f32x2{M, L};
-                }
-                __syncthreads();
-                const bool final = level || w0 / JOIN == w1 / JOIN;
-                for (int i = tid; i < items; i += 256) {
-                    const int r = i / (D / 4), d = i % (D / 4) * 4, u = r / rows, hh = r % rows;
-                    if (hh >= heads(sg * U + u)) continue;
-                    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-                    const float *src = a.part + (size_t)(u * DEC_HEADS + hh) * D + d;
-                    for (uint32_t p = 0; p < n; p += 8) {
-                        f32x4 v[8];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            v[j] = p + j < n ? remote4(src + at_piece(p + j) * prow * D) : f32x4{};
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x += (p + j < n ? fac[(p + j) * R + r] : 0.f) * v[j];
-                    }
-                    if (final) put(u, hh, d, x, ml[r].x, ml[r].y);
-                    else publish(a.part + (at_piece(0) * prow + u * DEC_HEADS + hh) * D + d, x);
-                }
-                if (final) break;
-                for (int r = tid; r < R; r += 256)
-                    publish(a.part_ml + (at_piece(0) * prow + r / rows * DEC_HEADS + r % rows) * 2, ml[r]);
-                first = w0 / JOIN * JOIN;
-                stride = JOIN;
-                n = w1 / JOIN - w0 / JOIN + 1;
-                count = a.arrived + 2 * gridDim.x + w0;
-            }
+        if (t0 == 0) {
+            const Piece pc = {b, sg, (int)blockIdx.x, (int)((unit + nt - 1) / share - blockIdx.x + 1)};
+            if (by_group) {
+                if (tid == 0) a.piece[b * ng + sg] = pc;
+            } else if (!whole) tail = pc;
         }
         pos = unit + t1;
         if (pos < hi) { // the next (sequence, heads)
@@ -391,15 +318,119 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
             }
         }
     }
+    if (!by_group && tid == 0) a.piece[blockIdx.x] = tail;
+}
+
+// The partial rows of a group that several runs share: out = sum_p f_p x_p / sum_p f_p l_p,
+// f_p = 2^(m_p - max m), in the pieces' order.  Up to JOIN_FEW pieces: a thread takes four elements of a
+// row through all of them.  More: a row at a time, a thread four elements of every PG-th piece, JOIN_B of
+// them under way.
+constexpr int JOIN_FEW = 16, JOIN_B = 16;
+template <typename T, int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_wg) {
+    constexpr int TPR = D / 4, PG = THREADS / TPR;
+    __shared__ float s_f[DEC_MAX_WG];
+    __shared__ f32x4 s_x[PG][TPR];
+    const Piece pc = {ldc(&a.piece[blockIdx.x].b), ldc(&a.piece[blockIdx.x].sg), ldc(&a.piece[blockIdx.x].w0),
+                      ldc(&a.piece[blockIdx.x].n)};
+    const int n = pc.n;
+    if (n < 2) return;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS, U = DEC_WAVES >> a.wpu_shift;
+    const int rows = min(DEC_HEADS, a.group);
+    const int r0 = blockIdx.y * rows_per_wg, r1 = min(U * rows, r0 + rows_per_wg);
+    // row r of piece p: of the first workgroup the later slot, of the others the earlier one
+    auto slot = [&](int p) { return 2 * (size_t)(pc.w0 + p) + (p == 0 ? 1 : 0); };
+    auto place = [&](int r) { return r / rows * DEC_HEADS + r % rows; };
+    auto row = [&](int r, int p) { return slot(p) * (DEC_WAVES * DEC_HEADS) + place(r); };
+    // its query head, or -1 for a place that the last head block does not have
+    auto head = [&](int r) {
+        const int hb = pc.sg * U + r / rows, hh = r % rows;
+        return hh < a.group - hb % gb * DEC_HEADS ? hb / gb * a.group + hb % gb * DEC_HEADS + hh : -1;
+    };
+    if (n <= JOIN_FEW) {
+        for (int i = r0 * TPR + tid; i < r1 * TPR; i += THREADS) {
+            const int r = i / TPR, d = i % TPR * 4, h = head(r);
+            if (h < 0) continue;
+            f32x2 ml[JOIN_FEW];
+            f32x4 v[JOIN_FEW];
+#pragma unroll
+            for (int p = 0; p < JOIN_FEW; ++p) {
+                ml[p] = p < n ? ldg<f32x2>(a.part_ml + ml_at(a, place(r), slot(p))) : f32x2{-INFINITY, 0.f};
+                v[p] = p < n ? ldg<f32x4>(a.part + row(r, p) * D + d) : f32x4{};
+            }
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int p = 0; p < JOIN_FEW; ++p) M = fmaxf(M, ml[p].x);
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int p = 0; p < JOIN_FEW; ++p) {
+                const float f = exp2_(ml[p].x - base_of(M));
+                L += f * ml[p].y;
+                x += f * v[p];
+            }
+            put_row<T>(a, pc.b, h, D, d, x, M, L);
+        }
+        return;
+    }
+    const int pg = tid / TPR, d = tid % TPR * 4;
+    for (int r = r0; r < r1; ++r) {
+        const int h = head(r);
+        if (h < 0) continue;
+        f32x4 v[JOIN_B];
+        auto load = [&](int p) {
+#pragma unroll
+            for (int j = 0; j < JOIN_B; ++j)
+                v[j] = p + j * PG < n ? ldg<f32x4>(a.part + row(r, p + j * PG) * D + d) : f32x4{};
+        };
+        load(pg);
+        float M = -INFINITY, L = 0.f;
+        for (int p = lane; p < n; p += 64) M = fmaxf(M, ldg<f32x2>(a.part_ml + ml_at(a, place(r), slot(p))).x);
+        M = wave_max(M);
+        for (int p = lane; p < n; p += 64) {
+            const f32x2 ml = ldg<f32x2>(a.part_ml + ml_at(a, place(r), slot(p)));
+            const float f = exp2_(ml.x - base_of(M));
+            L += f * ml.y;
+            if (tid < 64) s_f[p] = f;
+        }
+        L = wave_sum(L);
+        lds_barrier();
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        for (int p = pg;;) {
+#pragma unroll
+            for (int j = 0; j < JOIN_B; ++j)
+                if (p + j * PG < n) x += s_f[p + j * PG] * v[j];
+            if ((p += JOIN_B * PG) >= n) break;
+            load(p);
+        }
+        s_x[pg][tid % TPR] = x;
+        lds_barrier();
+        if (pg == 0) {
+            for (int i = 1; i < PG; ++i) x += s_x[i][tid];
+            put_row<T>(a, pc.b, h, D, d, x, M, L);
+        }
+        lds_barrier(); // s_f and s_x are free again
+    }
+}
+
+template <typename T, int D>
+hipError_t decode_d(const AttnArgs &a, hipStream_t st) {
+    k_attn_decode<T, D><<<a.n_wg, 256, 0, st>>>(a);
+    // Few groups, so possibly many pieces each: one row a workgroup of 512.  Many, so two or three
+    // pieces of each mostly: the rows that 256 threads hold.
+    const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS, U = DEC_WAVES >> a.wpu_shift;
+    const int rows = U * (a.group < DEC_HEADS ? a.group : DEC_HEADS);
+    const int64_t groups = (int64_t)a.n_seqs * (a.hkv * gb / U);
+    const int x = groups <= a.n_wg ? (int)groups : a.n_wg, per = 1024 / D;
+    if (x * rows <= 512) k_attn_join<T, D, 512><<<dim3(x, rows), 512, 0, st>>>(a, 1);
+    else if (x * rows <= 2048) k_attn_join<T, D, 256><<<dim3(x, rows), 256, 0, st>>>(a, 1);
+    else k_attn_join<T, D, 256><<<dim3(x, (rows + per - 1) / per), 256, 0, st>>>(a, per);
+    return hipGetLastError();
 }
 
 template <typename T>
-hipError_t decode_d(const AttnArgs &a, int d, hipStream_t st) {
-    const unsigned grid = (unsigned)a.n_wg;
-    if (d == 64) k_attn_decode<T, 64><<<grid, 256, 0, st>>>(a);
-    else if (d == 128) k_attn_decode<T, 128><<<grid, 256, 0, st>>>(a);
-    else k_attn_decode<T, 256><<<grid, 256, 0, st>>>(a);
-    return hipGetLastError();
+hipError_t decode_t(const AttnArgs &a, int d, hipStream_t st) {
+    return d == 64 ? decode_d<T, 64>(a, st) : d == 128 ? decode_d<T, 128>(a, st) : decode_d<T, 256>(a, st);
 }
 
 } // namespace
@@ -412,7 +443,7 @@ hipError_t launch_attn_decode(const AttnArgs &args, int type, int d, hipStream_t
     a.wpu_shift = 2;
     if (hb % 4 == 0 && units >= 4 * a.n_wg) a.wpu_shift = 0;
     else if (hb % 2 == 0 && units >= 2 * a.n_wg) a.wpu_shift = 1;
-    return type == MOE_T_F16 ? decode_d<f16_t>(a, d, st) : decode_d<bf16_t>(a, d, st);
+    return type == MOE_T_F16 ? decode_t<f16_t>(a, d, st) : decode_t<bf16_t>(a, d, st);
 }
 
 } // namespace moe
