@@ -131,7 +131,7 @@ moe_status attn_call(const char *fn, moe_attn *a, const moe_kv_cache *kv, const 
     OnDevice on(a->device);
     hipError_t he = on.he;
     if (he == hipSuccess)
-        he = c.row_start ? launch_attn(c, a->cfg.type, a->cfg.head_dim, (hipStream_t)stream)
+        he = c.row_start ? launch_attn_prompt(c, a->cfg.type, a->cfg.head_dim, (hipStream_t)stream)
                          : launch_attn_decode(c, a->cfg.type, a->cfg.head_dim, (hipStream_t)stream);
     if (he != hipSuccess) return fail(MOE_EHIP, "%s: launch: %s", fn, hipGetErrorString(he));
     return ok();

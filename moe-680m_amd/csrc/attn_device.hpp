@@ -92,6 +92,9 @@ __device__ __forceinline__ float wave_max(float x) {
     for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
     return x;
 }
+// A wave's own LDS writes are in place.
+__device__ __forceinline__ void lds_fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 } // namespace moe

@@ -42,6 +42,8 @@ constexpr int DEC_HEADS = 16;
 constexpr int DEC_WAVES = 4;
 constexpr int DEC_WAVE_TOK = 32;
 constexpr int DEC_MAX_WG = 1024;
+// Prompt: (token, head) rows of a workgroup.
+constexpr int PR_ROWS = 128;
 
 struct AppendArgs {
     const uint8_t *src[2];    // new keys, new values
@@ -52,7 +54,7 @@ struct AppendArgs {
 
 hipError_t launch_kv_append(const AppendArgs &a, int type, int in_type, int d, hipStream_t st);
 hipError_t launch_attn_decode(const AttnArgs &a, int type, int d, hipStream_t st);
-hipError_t launch_attn(const AttnArgs &a, int type, int d, hipStream_t st);
+hipError_t launch_attn_prompt(const AttnArgs &a, int type, int d, hipStream_t st);
 hipError_t launch_attn_flags(uint32_t *flags, uint32_t *dst, hipStream_t st);
 
 } // namespace moe

@@ -92,18 +92,20 @@ class Setup:
         """(o, bound, lse, lse_bound) in 64 bits; rows of no sequence stay NaN in o.
 
         bound, element by element, of a kernel that holds scores, maxima, sums and products in f32,
-        rounds each softmax weight to the type (f16: 2^15 above, so a weight under 2^-29 of the
-        largest loses absolutely at most 2^-40) and the result once:
+        rounds each softmax weight to the type and the result once:
           scores: f32 products are exact, their sum of d terms and the scaling by two more
             roundings are off by e_s <= (d + 4) 2^-24 scale sum |q_i k_i|;
           weights: e^s off by a factor of e_s + 2^-22 (base-2 exponential, its argument's
             subtraction under 2^-23 |s - m|), over the sum's, so twice that;
           sums of n weights or products: (n + 64) 2^-24 (every order of summation, the rescaling of a
             running maximum and the joining of pieces included), twice;
-          the weight's rounding: u = eps / 2 of the type; the result's: u |o|."""
+          the weight's rounding: u = eps / 2 of the type, and where f16 runs out of exponent half a step of
+            its smallest numbers, 2^-25, over what the largest weight is scaled to: 2^15 in the decode
+            form (2^-40), 2^7 at least in the prompt form (2^-32); the result's: u |o|."""
         scale = self.d ** -0.5 if scale is None else scale
         u = torch.finfo(self.type).eps / 2
         tiny = torch.finfo(self.type).smallest_normal * torch.finfo(self.type).eps / 2
+        lost = 2.0 ** -40 if self.rows is None else 2.0 ** -32
         group = self.hq // self.hkv
         o = torch.full((self.n_rows, self.hq, self.d), float("nan"), dtype=torch.float64)
         bound = torch.zeros_like(o)
@@ -129,7 +131,7 @@ class Setup:
             av = v.abs()
             mass = (w.unsqueeze(-1) * av).sum(1)
             bound[row] = (u * o[row].abs() + (u + off) * mass * (1 + u) + (w * e_w).unsqueeze(-1).mul(av).sum(1)
-                          + 2.0 ** -40 * av.sum(1) + tiny)
+                          + lost * av.sum(1) + tiny)
             lse[row] = torch.logsumexp(s, -1)
             lse_bound[row] = off.squeeze(-1) + 4 * EPS32 * (1 + lse[row].abs() + m.squeeze(-1).abs())
         return o, bound, lse, lse_bound
