@@ -92,8 +92,21 @@ __device__ __forceinline__ float wave_max(float x) {
     for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
     return x;
 }
-// A wave's own LDS writes are in place.
-__device__ __forceinline__ void lds_fence() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+#define MOE_LDS __attribute__((address_space(3)))
+// 16 bytes a lane straight to LDS: lane i's to lds + 16 i.  They are there behind lds_loaded() (and, for
+// other waves, a barrier).
+__device__ __forceinline__ void lds_load16(const uint8_t *base, uint32_t off, void *lds) {
+    __builtin_amdgcn_global_load_lds((const MOE_GLOBAL void *)((const MOE_GLOBAL uint8_t *)base + off), (MOE_LDS void *)lds,
+                                     16, 0, 0);
+}
+__device__ __forceinline__ void lds_loaded() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// The transposing LDS read: among 16 lanes, lane 4 j + c addresses elements 4c..4c+3 of row j, lane i gets
+// element i of rows 0..3.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ u32x2 lds_read_tr(const uint8_t *p) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((MOE_LDS s16x4 *)p));
+}
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 

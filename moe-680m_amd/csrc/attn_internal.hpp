@@ -42,8 +42,6 @@ constexpr int DEC_HEADS = 16;
 constexpr int DEC_WAVES = 4;
 constexpr int DEC_WAVE_TOK = 32;
 constexpr int DEC_MAX_WG = 1024;
-// Prompt: (token, head) rows of a workgroup.
-constexpr int PR_ROWS = 128;
 
 struct AppendArgs {
     const uint8_t *src[2];    // new keys, new values
