@@ -19,6 +19,7 @@ struct moe_attn {
     float *part_ml = nullptr;  // [2 n_wg][DEC_WAVES][DEC_HEADS][2]
     Piece *piece = nullptr;    // [n_wg]
     int n_wg = 0;              // workgroups of a decode launch
+    int n_cu = 0;              // compute units of the device
 };
 
 namespace {
@@ -128,6 +129,7 @@ moe_status attn_call(const char *fn, moe_attn *a, const moe_kv_cache *kv, const 
     c.part_ml = a->part_ml;
     c.piece = a->piece;
     c.n_wg = a->n_wg;
+    c.n_cu = a->n_cu;
     OnDevice on(a->device);
     hipError_t he = on.he;
     if (he == hipSuccess)
@@ -169,6 +171,7 @@ moe_status moe_attn_create(int device, const moe_attn_config *cfg, moe_attn **ou
     while ((1 << a->page_shift) < g.page_tokens) ++a->page_shift;
     int ncu = 0;
     if (hipDeviceGetAttribute(&ncu, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || ncu < 1) ncu = 1;
+    a->n_cu = ncu;
     a->n_wg = 2 * ncu < DEC_MAX_WG ? 2 * ncu : DEC_MAX_WG;
     struct Part {
         void **dst;

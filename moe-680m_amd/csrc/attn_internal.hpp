@@ -34,6 +34,7 @@ struct AttnArgs {
     float *part_ml;           // ... and each partial row's running maximum and sum
     Piece *piece;             // ... and the groups to join
     int n_wg;                 // workgroups of a decode launch
+    int n_cu;
     int wpu_shift;            // decode: log2 of the waves that share a unit
 };
 

@@ -52,21 +52,23 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w) {
     return w;
 }
 
-// One LDS read each of N fragments, READS instructions a fragment, ahead of the MFMAS products it serves,
-// DEPTH fragments early (the order that the compiler is told to keep; by itself it reads, waits, multiplies).
-template <int N, int READS, int MFMAS, int DEPTH>
-__device__ __forceinline__ void keep_reading() {
-    __builtin_amdgcn_sched_group_barrier(0x100, READS * DEPTH, 0);
+// Products of N fragments, each read from LDS DEPTH products before its own.  The order is kept as written
+// (by itself the compiler reads, waits, multiplies).
+template <int N, int DEPTH, typename Frag, typename Read, typename Product>
+__device__ __forceinline__ void products(Read read, Product product) {
+    Frag f[DEPTH];
 #pragma unroll
-    for (int i = 0; i < N - DEPTH; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, MFMAS, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    for (int i = 0; i < DEPTH; ++i) f[i] = read(i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        product(i, f[i % DEPTH]);
+        if (i + DEPTH < N) f[i % DEPTH] = read(i + DEPTH);
+        __builtin_amdgcn_sched_barrier(0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, MFMAS * DEPTH, 0);
 }
 
 template <typename T, int D, int NQ, int BN>
-__global__ __launch_bounds__(256, NQ * D > 256 ? 1 : 2) void k_attn_prompt(AttnArgs a) {
+__global__ __launch_bounds__(256, NQ * D >= 256 ? 1 : 2) void k_attn_prompt(AttnArgs a) {
     typedef Elem<T> E;
     typedef typename E::x8 x8;
     constexpr int KS = D / 16;           // products of a score tile
@@ -75,6 +77,7 @@ __global__ __launch_bounds__(256, NQ * D > 256 ? 1 : 2) void k_attn_prompt(AttnA
     constexpr int RI = 512 / D;          // tokens of one wave load
     constexpr int NL = BN / 4 / RI;      // loads of a wave and tile, for K and for V
     constexpr int ROWS = 128 * NQ;
+    constexpr int DEPTH = D == 64 ? 4 : 6; // fragments read ahead
     constexpr float SHIFT = E::SHIFT > 0.f ? 7.f : 0.f; // f16: 2^(SHIFT + LAZY) is in range
     __shared__ __attribute__((aligned(16))) T s_k[2][BN * D];
     __shared__ __attribute__((aligned(16))) T s_v[2][BN * D];
@@ -103,7 +106,10 @@ __global__ __launch_bounds__(256, NQ * D > 256 ? 1 : 2) void k_attn_prompt(AttnA
     const uint32_t nth = blockIdx.x / a.hkv;
     if (nth >= total) return;
     const int hk = blockIdx.x - nth * a.hkv;
-    const uint32_t want = total - 1 - nth;
+    uint32_t want = total - 1 - nth;
+    // All at work at once, two on some CUs: there the lighter one is to lie beside the heavier one.
+    const uint32_t first = a.n_cu / a.hkv; // (head groups of) tiles that take a CU each
+    if (D < 256 && total > first && total * a.hkv <= 2u * a.n_cu && nth >= first) want = nth - first;
     const int owner = __builtin_ctzll(__ballot(incl > want));
     uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), owner);
     int b = owner * per;
@@ -129,10 +135,9 @@ __global__ __launch_bounds__(256, NQ * D > 256 ? 1 : 2) void k_attn_prompt(AttnA
         return (int)(p < 0 ? 0 : p > cap ? cap : p);
     };
     const int64_t wf0 = f0 + wave * (32 * NQ);
-    const int64_t f_last = f0 + ROWS < nf ? f0 + ROWS : nf, w_last = wf0 + 32 * NQ < nf ? wf0 + 32 * NQ : nf;
+    const int64_t f_last = f0 + ROWS < nf ? f0 + ROWS : nf;
     const int ext = uniform(seen_by(f_last - 1));  // tokens that some row of the workgroup sees
     const int full = uniform(seen_by(f0));         // ... that all see
-    const int wave_ext = wf0 < nf ? uniform(seen_by(w_last - 1)) : 0;
     // a lane's rows: pair wf0 + 32 n + r; one behind the last reads the last one's query and sees nothing
     auto pair = [&](int n) { return wf0 + 32 * n + r; };
     auto q_at = [&](int n, int64_t stride) {
@@ -158,37 +163,41 @@ __global__ __launch_bounds__(256, NQ * D > 256 ? 1 : 2) void k_attn_prompt(AttnA
     const float scale = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);
 
     // ---- tiles
+    const int nt = (ext + BN - 1) / BN;
     const int32_t *pages = a.pages + b * a.pages_stride;
     const uint8_t *kb = a.k + 2 * hk * a.head_stride, *vb = a.v + 2 * hk * a.head_stride;
     const int ts2 = (int)(2 * a.token_stride), mask = (1 << a.page_shift) - 1;
+    // Lane i has the page of block i of the tile to be staged next (-1: none); okay: the blocks of the tile
+    // staged last that have a page of the cache, or no token to be seen.
     bool bad_page = false;
-    int have[NB]; // tokens of the blocks of the tile that is staged last
-    // Stage tile t: every wave loads its quarter, from one page.  Tokens that are not there are taken from a
-    // place that is (masked below).
-    auto stage = [&](int t, int buf) {
-        int64_t off = 0;
-        int n = 0;
-        const int blk = wave * NB / 4;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            const int key = t * BN + 16 * i;
-            int pg = 0;
-            have[i] = min(16, max(0, ext - key));
-            if (have[i] > 0) {
-                pg = ldc(pages + (key >> a.page_shift));
-                if ((unsigned)pg >= (unsigned)a.n_pages) bad_page = true, pg = 0, have[i] = 0;
-            }
-            if (i == blk) {
-                off = 2 * (pg * a.page_stride + (key & mask) * a.token_stride);
-                n = have[i];
-            }
-        }
+    uint32_t okay = 0;
+    auto look_up = [&](int t) {
+        const int key = t * BN + 16 * lane;
+        return lane < NB && key < ext ? ldg<int>(pages + (key >> a.page_shift)) : -1;
+    };
+    int pg_next = look_up(0);
+    int64_t off = 0; // of this wave's quarter of the tile: one block's, or a part of it; tokens there
+    int toks = 0;
+    auto stage = [&](int t) {
+        const int blk = wave * NB / 4, key = t * BN + 16 * blk;
+        const uint64_t in = __ballot((unsigned)pg_next < (unsigned)a.n_pages);
+        const uint64_t none = __ballot(t * BN + 16 * lane >= ext);
+        okay = (uint32_t)(in | none);
+        bad_page |= (okay & ((1u << NB) - 1)) != (1u << NB) - 1;
+        const bool here = in >> blk & 1;
+        const int pg = here ? __builtin_amdgcn_readlane(pg_next, blk) : 0;
+        toks = here ? min(16, ext - key) : 0;
+        off = 2 * (pg * a.page_stride + (key & mask) * a.token_stride);
+        if (t + 1 < nt) pg_next = look_up(t + 1);
+    };
+    // Every wave loads its quarter.  Tokens that are not there are taken from a place that is (masked below).
+    auto stage_load = [&](const uint8_t *base, T *lds, bool values) {
 #pragma unroll
         for (int p = 0; p < NL; ++p) {
             const int key = (wave * NL + p) * RI + lane / (D / 8), ch = lane % (D / 8); // of the tile
-            const int tok = max(0, min(key & 15, n - 1));
-            lds_load16(kb + off, (uint32_t)(tok * ts2 + (ch ^ (key & 7)) * 16), s_k[buf] + (wave * NL + p) * 512);
-            lds_load16(vb + off, (uint32_t)(tok * ts2 + (ch ^ (2 * (key & 3))) * 16), s_v[buf] + (wave * NL + p) * 512);
+            const int tok = max(0, min(key & 15, toks - 1));
+            lds_load16(base + off, (uint32_t)(tok * ts2 + (ch ^ (values ? 2 * (key & 3) : key & 7)) * 16),
+                       lds + (wave * NL + p) * 512);
         }
     };
 
@@ -210,51 +219,63 @@ __global__ __launch_bounds__(256, NQ * D > 256 ? 1 : 2) void k_attn_prompt(AttnA
         vo[1] = vo[0] ^ 64;
     }
 
-    const int nt = (ext + BN - 1) / BN;
-    if (nt > 0) stage(0, 0);
-    for (int t = 0; t < nt; ++t) {
-        const int buf = t & 1;
-        const uint8_t *lk = (const uint8_t *)s_k[buf], *lv = (const uint8_t *)s_v[buf];
-        int hv[NB];
-        bool part = (t + 1) * BN > full; // a tile that some row does not see all of
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            hv[i] = have[i];
-            part |= hv[i] < 16;
-        }
-        lds_loaded();
-        __syncthreads(); // tile t is there, and nobody works on tile t - 1
-        // A value that a row does not see meets a weight of 0, which an infinity or NaN would survive: in
-        // such a tile those are 0 for the products, and the rows that see them get them at the end.
-        if (part) {
-            bool bad = false;
-#pragma unroll 1
-            for (int i = tid; i < BN * D / 8; i += 256) {
-                u32x4 *p = (u32x4 *)s_v[buf] + i;
-                u32x4 w = *p;
-                bool any = false;
-                for (int j = 0; j < 4; ++j) any |= not_finite<T>(w[j]);
-                if (any) {
-                    for (int j = 0; j < 4; ++j) w[j] = finite_only<T>(w[j]);
-                    *p = w;
-                    bad = true;
+    if (nt > 0) {
+        stage(0);
+        stage_load(kb, s_k[0], false);
+        stage_load(vb, s_v[0], true);
+    }
+    bool fresh = true, part = false;
+    uint32_t ok = 0;
+    for (int t = 0; t < nt;) {
+        // Tiles until a row's maximum grows past what its weights allow for; then the outputs are rescaled
+        // and the tile's scores computed again.  (Two loops, so that the inner one's outputs are the
+        // products' own and stay where those put them.)
+        float mx[NQ];
+        for (;;) {
+            const int buf = t & 1;
+            const uint8_t *lk = (const uint8_t *)s_k[buf], *lv = (const uint8_t *)s_v[buf];
+            if (fresh) {
+                ok = okay;
+                // a tile that some row does not see all of
+                part = (t + 1) * BN > full || (ok & ((1u << NB) - 1)) != (1u << NB) - 1;
+                lds_loaded();
+                __syncthreads(); // tile t is there, and nobody works on tile t - 1
+                // A value that a row does not see meets a weight of 0, which an infinity or NaN would survive:
+                                // in such a tile those are 0 for the products, and the rows that see them get them at the end.
+                                if (part) {
+                                    bool bad = false;
+                #pragma unroll 1
+                                    for (int i = tid; i < BN * D / 8; i += 256) {
+                                        u32x4 *p = (u32x4 *)s_v[buf] + i;
+                                        u32x4 w = *p;
+                                        bool any = false;
+                                        for (int j = 0; j < 4; ++j) any |= not_finite<T>(w[j]);
+                                        if (any) {
+                                            for (int j = 0; j < 4; ++j) w[j] = finite_only<T>(w[j]);
+                                            *p = w;
+                                            bad = true;
+                                        }
+                                    }
+                                    if (bad) s_bad = 1;
+                                    __syncthreads();
+                                }
+                if (t + 1 < nt) {
+                    stage(t + 1);
+                    stage_load(kb, s_k[buf ^ 1], false);
+                    stage_load(vb, s_v[buf ^ 1], true);
                 }
             }
-            if (bad) s_bad = 1;
-            __syncthreads();
-        }
-        if (t + 1 < nt) stage(t + 1, buf ^ 1);
-        if (D == 256 || t * BN < wave_ext) { // (at D = 256 the branch costs a copy of all outputs)
             f32x16 s[NQ][NS];
+            auto read_k = [&](int x) { // the score tiles in turn: two chains of sums
+                const int i = x % NS, k = x / NS;
+                return *(const x8 *)(lk + ko[k & 3] + i * (32 * D * 2) + (k >> 2) * 128);
+            };
+            auto mul_k = [&](int x, x8 kf) {
+                const int i = x % NS, k = x / NS;
 #pragma unroll
-            for (int i = 0; i < NS; ++i)
-#pragma unroll
-                for (int k = 0; k < KS; ++k) {
-                    const x8 kf = *(const x8 *)(lk + ko[k & 3] + i * (32 * D * 2) + (k >> 2) * 128);
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) s[n][i] = E::mfma32(kf, qf[n][k], k ? s[n][i] : f32x16{});
-                }
-            keep_reading<NS * KS, 1, NQ, 4>();
+                for (int n = 0; n < NQ; ++n) s[n][i] = E::mfma32(kf, qf[n][k], k ? s[n][i] : f32x16{});
+            };
+            products<NS * KS, DEPTH, x8>(read_k, mul_k);
             if (part)
 #pragma unroll
                 for (int n = 0; n < NQ; ++n)
@@ -263,25 +284,24 @@ __global__ __launch_bounds__(256, NQ * D > 256 ? 1 : 2) void k_attn_prompt(AttnA
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
                             const int key = 32 * i + 8 * (j >> 2) + 4 * h + (j & 3);
-                            if (t * BN + key >= seen[n] || (key & 15) >= hv[2 * i + (j >> 3)]) s[n][i][j] = -INFINITY;
+                            if (t * BN + key >= seen[n] || !(ok >> (2 * i + (j >> 3)) & 1)) s[n][i][j] = -INFINITY;
                         }
-            u32x4 pw[NQ][2 * NS]; // the weights, in P^T's operand layout
+            bool grows = false;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-                float mx = s[n][0][0];
+                mx[n] = s[n][0][0];
 #pragma unroll
                 for (int i = 0; i < NS; ++i)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[n][i][j]);
-                mx = fmaxf(mx, __shfl_xor(mx, 32)) * scale;
-                if (__any(mx > m[n] + LAZY)) {
-                    const float mn = fmaxf(m[n], mx);
-                    const float alpha = exp2_(m[n] - base_of(mn));
-                    m[n] = mn;
-                    l[n] *= alpha;
+                    for (int j = 0; j < 16; ++j) mx[n] = fmaxf(mx[n], s[n][i][j]);
+                mx[n] = fmaxf(mx[n], __shfl_xor(mx[n], 32)) * scale;
+                grows |= mx[n] > m[n] + LAZY;
+            }
+            fresh = !__any(grows);
+            if (!fresh) break;
+            u32x4 pw[NQ][2 * NS]; // the weights, in P^T's operand layout
 #pragma unroll
-                    for (int i = 0; i < D / 32; ++i) o[n][i] *= alpha;
-                }
+            for (int n = 0; n < NQ; ++n) {
                 const float base = base_of(m[n]) - SHIFT;
                 float sum = 0.f;
 #pragma unroll
@@ -295,18 +315,30 @@ __global__ __launch_bounds__(256, NQ * D > 256 ? 1 : 2) void k_attn_prompt(AttnA
                     }
                 l[n] += sum;
             }
+            auto read_v = [&](int x) {
+                const int k = x / (D / 32), i = x % (D / 32);
+                const uint8_t *p = lv + vo[i & 1] + k * (16 * D * 2) + (i >> 1) * 128;
+                const u32x2 v0 = lds_read_tr(p), v1 = lds_read_tr(p + 8 * D * 2);
+                return __builtin_bit_cast(x8, (u32x4{v0.x, v0.y, v1.x, v1.y}));
+            };
+            auto mul_v = [&](int x, x8 vf) {
+                const int k = x / (D / 32), i = x % (D / 32);
 #pragma unroll
-            for (int k = 0; k < 2 * NS; ++k)
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    const uint8_t *p = lv + vo[i & 1] + k * (16 * D * 2) + (i >> 1) * 128;
-                    const u32x2 v0 = lds_read_tr(p), v1 = lds_read_tr(p + 8 * D * 2);
-                    const x8 vf = __builtin_bit_cast(x8, (u32x4{v0.x, v0.y, v1.x, v1.y}));
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) o[n][i] = E::mfma32(vf, __builtin_bit_cast(x8, pw[n][k]), o[n][i]);
-                }
-            keep_reading<NS * D / 16, 2, NQ, 4>();
+                for (int n = 0; n < NQ; ++n) o[n][i] = E::mfma32(vf, __builtin_bit_cast(x8, pw[n][k]), o[n][i]);
+            };
+            products<NS * D / 16, DEPTH, x8>(read_v, mul_v);
+            if (++t == nt) break;
         }
+        if (t < nt)
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                const float mn = fmaxf(m[n], mx[n]);
+                const float alpha = exp2_(m[n] - base_of(mn));
+                m[n] = mn;
+                l[n] *= alpha;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) o[n][i] *= alpha;
+            }
     }
     if (bad_page && lane == 0) raise(a.flags, MOE_DEVFLAG_BAD_PAGE);
 
@@ -362,7 +394,7 @@ hipError_t prompt_t(const AttnArgs &a, int d, hipStream_t st) {
     const unsigned grid = (unsigned)(tiles * a.hkv);
     if (d == 64) k_attn_prompt<T, 64, 1, 64><<<grid, 256, 0, st>>>(a);
     else if (d == 128) k_attn_prompt<T, 128, 1, 64><<<grid, 256, 0, st>>>(a);
-    else k_attn_prompt<T, 256, 1, 32><<<grid, 256, 0, st>>>(a);
+    else k_attn_prompt<T, 256, 1, 64><<<grid, 256, 0, st>>>(a);
     return hipGetLastError();
 }
 
