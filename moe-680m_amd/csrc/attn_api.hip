@@ -15,8 +15,9 @@ struct moe_attn {
     int page_shift = 0;
     void *arena = nullptr;     // one device allocation, carved below
     uint32_t *flags = nullptr; // sticky device flags
-    float *part = nullptr;     // decode partials: [2 n_wg][DEC_WAVES][DEC_HEADS][head_dim]
-    float *part_ml = nullptr;  // [2 n_wg][DEC_WAVES][DEC_HEADS][2]
+    float *part = nullptr;     // partial rows: [part_rows][head_dim]
+    float *part_ml = nullptr;  // ... and each one's maximum and sum: [part_rows][2]
+    int64_t part_rows = 0;
     Piece *piece = nullptr;    // [n_wg]
     int n_wg = 0;              // workgroups of a decode launch
     int n_cu = 0;              // compute units of the device
@@ -127,6 +128,7 @@ moe_status attn_call(const char *fn, moe_attn *a, const moe_kv_cache *kv, const 
     c.scale_log2 = (float)(scale * 1.4426950408889634);
     c.part = a->part;
     c.part_ml = a->part_ml;
+    c.part_rows = a->part_rows;
     c.piece = a->piece;
     c.n_wg = a->n_wg;
     c.n_cu = a->n_cu;
@@ -173,14 +175,18 @@ moe_status moe_attn_create(int device, const moe_attn_config *cfg, moe_attn **ou
     if (hipDeviceGetAttribute(&ncu, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || ncu < 1) ncu = 1;
     a->n_cu = ncu;
     a->n_wg = 2 * ncu < DEC_MAX_WG ? 2 * ncu : DEC_MAX_WG;
+    // decode: two slots a workgroup; prompt: 3.5 pieces for each place on the card at most (prompt_d)
+    const int64_t dec_rows = (int64_t)a->n_wg * 2 * DEC_WAVES * DEC_HEADS;
+    const int64_t prompt_rows = (int64_t)ncu * (g.head_dim == 256 ? 1 : 2) * 7 / 2 * PR_ROWS;
+    a->part_rows = dec_rows > prompt_rows ? dec_rows : prompt_rows;
     struct Part {
         void **dst;
         size_t bytes;
     } parts[] = {
         {(void **)&a->flags, 256},
         {(void **)&a->piece, (size_t)a->n_wg * sizeof(Piece)},
-        {(void **)&a->part_ml, (size_t)a->n_wg * 2 * DEC_WAVES * DEC_HEADS * 2 * 4},
-        {(void **)&a->part, (size_t)a->n_wg * 2 * DEC_WAVES * DEC_HEADS * g.head_dim * 4},
+        {(void **)&a->part_ml, (size_t)a->part_rows * 2 * 4},
+        {(void **)&a->part, (size_t)a->part_rows * g.head_dim * 4},
     };
     size_t total = 0;
     for (auto &p : parts) total += (p.bytes + 255) / 256 * 256;

@@ -110,4 +110,18 @@ __device__ __forceinline__ u32x2 lds_read_tr(const uint8_t *p) {
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// Four elements of a finished row: x / L, and with the first ones the log of the sum; the weights were
+// 2^(score - M + shift).
+template <typename T, typename Args>
+__device__ __forceinline__ void put_row(const Args &a, int row, int h, int D, int d, f32x4 x, float M, float L,
+                                        float shift) {
+    typedef Elem<T> E;
+    const float inv = 1.f / L;
+    x = L == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : x * inv;
+    *(u32x2 *)((T *)a.o + row * a.o_stride + (int64_t)h * D + d) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+    if (a.lse && d == 0)
+        a.lse[(int64_t)row * a.hq + h] =
+            L == 0.f ? -INFINITY : (base_of(M) - shift + __log2f(L)) * 0.69314718055994531f;
+}
+
 } // namespace moe

@@ -36,6 +36,8 @@ struct AttnArgs {
     int n_wg;                 // workgroups of a decode launch
     int n_cu;
     int wpu_shift;            // decode: log2 of the waves that share a unit
+    int splits;               // prompt: pieces of the longest rows
+    int64_t part_rows;        // rows that part and part_ml hold
 };
 
 // Decode: heads of one matrix tile, waves of a workgroup, tokens of a wave's step.
@@ -43,6 +45,8 @@ constexpr int DEC_HEADS = 16;
 constexpr int DEC_WAVES = 4;
 constexpr int DEC_WAVE_TOK = 32;
 constexpr int DEC_MAX_WG = 1024;
+// Prompt: (token, head) rows of a workgroup.
+constexpr int PR_ROWS = 128;
 
 struct AppendArgs {
     const uint8_t *src[2];    // new keys, new values

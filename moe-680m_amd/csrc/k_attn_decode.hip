@@ -43,18 +43,6 @@ __device__ __forceinline__ size_t ml_at(const Args &a, int place, size_t slot) {
     return (size_t)place * (4 * a.n_wg) + 2 * slot;
 }
 
-// Four elements of a finished row: x / L, and with the first ones the log of the sum.
-template <typename T, typename Args>
-__device__ __forceinline__ void put_row(const Args &a, int b, int h, int D, int d, f32x4 x, float M, float L) {
-    typedef Elem<T> E;
-    const float inv = 1.f / L;
-    x = L == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : x * inv;
-    *(u32x2 *)((T *)a.o + b * a.o_stride + (int64_t)h * D + d) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
-    if (a.lse && d == 0)
-        a.lse[(int64_t)b * a.hq + h] =
-            L == 0.f ? -INFINITY : (base_of(M) - E::SHIFT + __log2f(L)) * 0.69314718055994531f;
-}
-
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
     typedef Elem<T> E;
@@ -295,7 +283,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
                     L += f * ml[w].y;
                     x += f * y[w];
                 }
-            if (whole) put_row<T>(a, b, head0(sg * U + u) + hh, D, d, x, M, L);
+            if (whole) put_row<T>(a, b, head0(sg * U + u) + hh, D, d, x, M, L, E::SHIFT);
             else {
                 *(f32x4 *)(a.part + (slot * ROWS + u * DEC_HEADS + hh) * D + d) = x;
                 if (d == 0) *(f32x2 *)(a.part_ml + ml_at(a, u * DEC_HEADS + hh, slot)) = f32x2{M, L};
@@ -369,7 +357,7 @@ __global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_
                 L += f * ml[p].y;
                 x += f * v[p];
             }
-            put_row<T>(a, pc.b, h, D, d, x, M, L);
+            put_row<T>(a, pc.b, h, D, d, x, M, L, Elem<T>::SHIFT);
         }
         return;
     }
@@ -407,7 +395,7 @@ __global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_
         lds_barrier();
         if (pg == 0) {
             for (int i = 1; i < PG; ++i) x += s_x[i][tid];
-            put_row<T>(a, pc.b, h, D, d, x, M, L);
+            put_row<T>(a, pc.b, h, D, d, x, M, L, Elem<T>::SHIFT);
         }
         lds_barrier(); // s_f and s_x are free again
     }

@@ -4,9 +4,9 @@
 //   p_i the row's position (kv_len - rows + i)
 //
 // Bound by the matrix cores: 4 D operations for each (row, head, seen token).  A workgroup's rows are
-// 128 NQ (token, head) pairs of one key-value head, the heads of a token side by side, so the
+// PR_ROWS (token, head) pairs of one key-value head, the heads of a token side by side, so the
 // group's heads share each tile of K and V and the causal edge crosses few of them.
-//   * A wave takes NQ blocks of 32 rows, a row to a lane pair:
+//   * A wave takes 32 rows, a row to a lane pair:
 //       S^T[token][row] = K Q^T      32x32x16 products; a row's scores lie in the lanes r and r + 32,
 //                                    so maximum, sum and rescaling are a lane's own (and one swap)
 //       O^T[d][row] += V^T P^T       S^T's register layout is P^T's operand layout with the tokens of 16
@@ -16,16 +16,20 @@
 //     load: of 16 lanes, lane 4 j + c gives the address of elements 4c..4c+3 of token j, lane d gets
 //     element d of tokens 0..3.  A row's 16-byte chunks are stored at chunk ^ f(token), f = token & 7 for K
 //     and 2 (token & 3) for V, so that all reads are free of bank conflicts.
-//   * A fragment read from LDS serves the NQ row blocks of a wave.
 //   * The running maximum is only raised when a row's new one exceeds it by more than 2^8: until then
 //     the weights stay below 2^(8 + SHIFT) and no output is rescaled.
+//   * Too few rows to fill the card (a piece of a prompt over a long cache, short prompts): the tokens of
+//     the longest rows are cut into pieces, whose partial rows a second launch joins.
 #include "attn_device.hpp"
 
 namespace moe {
 
 namespace {
 
-constexpr float LAZY = 8.f;     // log2 of what a weight may exceed 1 by
+constexpr int BN = 64;           // tokens of a tile
+constexpr float LAZY = 8.f;      // log2 of what a weight may exceed 1 by
+constexpr int PR_MIN_CHUNK = 4;  // tiles of a piece at least
+constexpr int PR_MAX_SPLITS = 64;
 
 struct Rows {
     int r0, n;
@@ -36,6 +40,12 @@ __device__ __forceinline__ Rows seq_rows(const AttnArgs &a, int b) {
     const int s = a.row_start[b], e = a.row_start[b + 1];
     const int r0 = min(max(s, 0), a.n_rows), r1 = min(max(e, r0), a.n_rows);
     return {r0, r1 - r0, r0 != s || r1 != e};
+}
+
+// Tokens that the f-th (token, head) pair's row of a sequence sees, its first row's position given.
+__device__ __forceinline__ int seen_by(const AttnArgs &a, int64_t first_pos, int64_t f) {
+    const int64_t p = first_pos + f / a.group + 1, cap = (int64_t)a.max_pages << a.page_shift;
+    return (int)(p < 0 ? 0 : p > cap ? cap : p);
 }
 
 // Of two elements in a word: whether one is an infinity or NaN; the word with those as 0.
@@ -67,95 +77,123 @@ __device__ __forceinline__ void products(Read read, Product product) {
     }
 }
 
-template <typename T, int D, int NQ, int BN>
-__global__ __launch_bounds__(256, NQ * D >= 256 ? 1 : 2) void k_attn_prompt(AttnArgs a) {
-    typedef Elem<T> E;
-    typedef typename E::x8 x8;
-    constexpr int KS = D / 16;           // products of a score tile
-    constexpr int NB = BN / 16;          // blocks of 16 tokens, each in one page
-    constexpr int NS = BN / 32;          // score tiles
-    constexpr int RI = 512 / D;          // tokens of one wave load
-    constexpr int NL = BN / 4 / RI;      // loads of a wave and tile, for K and for V
-    constexpr int ROWS = 128 * NQ;
-    constexpr int DEPTH = D == 64 ? 4 : 6; // fragments read ahead
-    constexpr float SHIFT = E::SHIFT > 0.f ? 7.f : 0.f; // f16: 2^(SHIFT + LAZY) is in range
-    __shared__ __attribute__((aligned(16))) T s_k[2][BN * D];
-    __shared__ __attribute__((aligned(16))) T s_v[2][BN * D];
-    __shared__ int s_bad;
+// A workgroup's place: PR_ROWS (token, head) pairs of sequence b, from its f0-th of nf on, of which the
+// last one sees ext tokens and the first one `full`; pieces of them, `chunk` tiles each.
+struct Place {
+    int b, r0, hk;
+    int64_t f0, nf, first_pos; // of the sequence's first row
+    int ext, full, chunk;
+};
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-    const int r = lane & 31, h = lane >> 5;
+// Place number blockIdx.x; false where there is none.  Tile numbers run over the sequences, the last one
+// first (it sees the most tokens); the key-value head is the fastest index, so that a head's tiles
+// share an XCD's L2.
+__device__ __forceinline__ bool find_place(const AttnArgs &a, int lane, bool snake, bool flag, Place &pl) {
     const int cap = a.max_pages << a.page_shift;
-
-    // ---- this workgroup's rows: tile numbers run over the sequences, the last one first (it sees the
-    // most tokens); the key-value head is the fastest index, so that a head's tiles share an XCD's L2
     const int per = (a.n_seqs + 63) / 64;
+    auto tiles = [&](int n) { return (uint32_t)(((int64_t)n * a.group + PR_ROWS - 1) / PR_ROWS); };
     uint32_t mine = 0;
-    bool bad_rows = false;
+    int most = 0; // tokens that a row sees
+    bool bad = false;
     for (int i = 0; i < per; ++i) {
         const int b = lane * per + i;
         if (b < a.n_seqs) {
             const Rows w = seq_rows(a, b);
-            bad_rows |= w.bad;
-            mine += (uint32_t)(((int64_t)w.n * a.group + ROWS - 1) / ROWS);
+            bad |= w.bad;
+            mine += tiles(w.n);
+            if (w.n > 0) {
+                const int len = a.kv_len[b];
+                bad |= len < 0 || len > cap;
+                most = max(most, min(len, cap));
+            }
         }
     }
-    if (blockIdx.x == 0 && bad_rows) raise(a.flags, MOE_DEVFLAG_BAD_SEQ);
+    if (flag && bad) raise(a.flags, MOE_DEVFLAG_BAD_SEQ);
     const uint32_t incl = wave_scan(mine);
     const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
     const uint32_t nth = blockIdx.x / a.hkv;
-    if (nth >= total) return;
-    const int hk = blockIdx.x - nth * a.hkv;
+    if (nth >= total) return false;
     uint32_t want = total - 1 - nth;
     // All at work at once, two on some CUs: there the lighter one is to lie beside the heavier one.
     const uint32_t first = a.n_cu / a.hkv; // (head groups of) tiles that take a CU each
-    if (D < 256 && total > first && total * a.hkv <= 2u * a.n_cu && nth >= first) want = nth - first;
+    if (snake && total > first && total * a.hkv <= 2u * a.n_cu && nth >= first) want = nth - first;
     const int owner = __builtin_ctzll(__ballot(incl > want));
     uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), owner);
     int b = owner * per;
     Rows sr;
     for (;; ++b) {
         sr = seq_rows(a, uniform(b));
-        const uint32_t n = (uint32_t)(((int64_t)sr.n * a.group + ROWS - 1) / ROWS);
+        const uint32_t n = tiles(sr.n);
         if (want < at + n) break;
         at += n;
     }
-    b = uniform(b);
-    sr.r0 = uniform(sr.r0);
-    sr.n = uniform(sr.n);
+    pl.b = uniform(b);
+    pl.r0 = uniform(sr.r0);
+    pl.hk = blockIdx.x - nth * a.hkv;
+    pl.f0 = (int64_t)(want - at) * PR_ROWS;
+    pl.nf = (int64_t)uniform(sr.n) * a.group;
+    pl.first_pos = (int64_t)ldc(a.kv_len + pl.b) - ldc(a.row_start + pl.b + 1) + pl.r0;
+    pl.full = uniform(seen_by(a, pl.first_pos, pl.f0));
+    pl.ext = uniform(seen_by(a, pl.first_pos, min(pl.f0 + PR_ROWS, pl.nf) - 1));
+    pl.chunk = 1 << 30;
+    if (a.splits > 1) {
+        for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
+        pl.chunk = uniform(max(PR_MIN_CHUNK, ((most + BN - 1) / BN + a.splits - 1) / a.splits));
+    }
+    return true;
+}
+
+// Partial rows of piece `piece` of place blockIdx.x.
+__device__ __forceinline__ size_t part_row(const AttnArgs &a, int piece) {
+    return ((size_t)blockIdx.x * a.splits + piece) * PR_ROWS;
+}
+
+// f16: 2^(SHIFT + LAZY) is in range.
+template <typename T>
+constexpr float SHIFT = Elem<T>::SHIFT > 0.f ? 7.f : 0.f;
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs a) {
+    typedef Elem<T> E;
+    typedef typename E::x8 x8;
+    constexpr int KS = D / 16;             // products of a score tile
+    constexpr int NB = BN / 16;            // blocks of 16 tokens, each in one page: one a wave
+    constexpr int NS = BN / 32;            // score tiles
+    constexpr int RI = 512 / D;            // tokens of one wave load
+    constexpr int NL = 16 / RI;            // loads of a wave and tile, for K and for V
+    constexpr int DEPTH = D == 64 ? 4 : 6; // fragments read ahead
+    constexpr uint32_t ALL = (1u << NB) - 1;
+    static_assert(NB == 4, "a block a wave");
+    __shared__ __attribute__((aligned(16))) T s_k[2][BN * D];
+    __shared__ __attribute__((aligned(16))) T s_v[2][BN * D];
+    __shared__ int s_bad;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int r = lane & 31, h = lane >> 5;
+    Place pl;
+    if (!find_place(a, lane, D < 256, blockIdx.x == 0 && blockIdx.y == 0 && wave == 0, pl)) return;
+    // this piece's tiles [t, nt); the first one also where no token is seen, to write the rows
+    const int tiles = (pl.ext + BN - 1) / BN, first_t = (int)min((int64_t)blockIdx.y * pl.chunk, (int64_t)1 << 30);
+    if (blockIdx.y > 0 && first_t >= tiles) return;
+    const int nt = min(tiles, first_t + pl.chunk), ext = pl.ext;
+    const bool whole = tiles <= pl.chunk;
     if (tid == 0) s_bad = 0;
 
-    // ---- rows: number f of the sequence's (token, head) pairs, position
-    const int64_t f0 = (int64_t)(want - at) * ROWS, nf = (int64_t)sr.n * a.group;
-    const int len = ldc(a.kv_len + b);
-    if ((len < 0 || len > cap) && tid == 0) raise(a.flags, MOE_DEVFLAG_BAD_SEQ);
-    const int64_t first_pos = (int64_t)len - ldc(a.row_start + b + 1) + sr.r0; // of the sequence's first row
-    auto seen_by = [&](int64_t f) { // tokens that pair f's row sees
-        const int64_t p = first_pos + f / a.group + 1;
-        return (int)(p < 0 ? 0 : p > cap ? cap : p);
-    };
-    const int64_t wf0 = f0 + wave * (32 * NQ);
-    const int64_t f_last = f0 + ROWS < nf ? f0 + ROWS : nf;
-    const int ext = uniform(seen_by(f_last - 1));  // tokens that some row of the workgroup sees
-    const int full = uniform(seen_by(f0));         // ... that all see
-    // a lane's rows: pair wf0 + 32 n + r; one behind the last reads the last one's query and sees nothing
-    auto pair = [&](int n) { return wf0 + 32 * n + r; };
-    auto q_at = [&](int n, int64_t stride) {
-        const int64_t f = pair(n) < nf ? pair(n) : nf - 1, tok = f / a.group;
-        return (sr.r0 + tok) * stride + (hk * a.group + (f - tok * a.group)) * D;
-    };
-    int seen[NQ];
-    x8 qf[NQ][KS];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        seen[n] = pair(n) < nf ? seen_by(pair(n)) : 0;
-        const T *q = (const T *)a.q + q_at(n, a.q_stride) + h * 8;
+    // this lane's row; one behind the last reads the last one's query and sees nothing
+    const int64_t pair = pl.f0 + wave * 32 + r;
+    const bool valid = pair < pl.nf;
+    const int tok = (int)((valid ? pair : pl.nf - 1) / a.group);
+    const int row = pl.r0 + tok, head = pl.hk * a.group + (int)((valid ? pair : pl.nf - 1) - (int64_t)tok * a.group);
+    const int seen = valid ? seen_by(a, pl.first_pos, pair) : 0;
+    x8 qf[KS];
+    {
+        const T *q = (const T *)a.q + row * a.q_stride + head * D + h * 8;
         const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u; // a negative scale: -q, exactly
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             u32x4 w = ldg<u32x4>(q + k * 16);
             for (int i = 0; i < 4; ++i) w[i] ^= flip;
-            qf[n][k] = __builtin_bit_cast(x8, w);
+            qf[k] = __builtin_bit_cast(x8, w);
         }
     }
     // Scale 0: the smallest normal number, so that -inf (not seen) stays -inf; any finite score times it
@@ -163,9 +201,8 @@ __global__ __launch_bounds__(256, NQ * D >= 256 ? 1 : 2) void k_attn_prompt(Attn
     const float scale = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);
 
     // ---- tiles
-    const int nt = (ext + BN - 1) / BN;
-    const int32_t *pages = a.pages + b * a.pages_stride;
-    const uint8_t *kb = a.k + 2 * hk * a.head_stride, *vb = a.v + 2 * hk * a.head_stride;
+    const int32_t *pages = a.pages + pl.b * a.pages_stride;
+    const uint8_t *kb = a.k + 2 * pl.hk * a.head_stride, *vb = a.v + 2 * pl.hk * a.head_stride;
     const int ts2 = (int)(2 * a.token_stride), mask = (1 << a.page_shift) - 1;
     // Lane i has the page of block i of the tile to be staged next (-1: none); okay: the blocks of the tile
     // staged last that have a page of the cache, or no token to be seen.
@@ -175,41 +212,36 @@ __global__ __launch_bounds__(256, NQ * D >= 256 ? 1 : 2) void k_attn_prompt(Attn
         const int key = t * BN + 16 * lane;
         return lane < NB && key < ext ? ldg<int>(pages + (key >> a.page_shift)) : -1;
     };
-    int pg_next = look_up(0);
-    int64_t off = 0; // of this wave's quarter of the tile: one block's, or a part of it; tokens there
+    int pg_next = look_up(first_t);
+    int64_t off = 0; // of this wave's block of the tile; tokens there
     int toks = 0;
     auto stage = [&](int t) {
-        const int blk = wave * NB / 4, key = t * BN + 16 * blk;
+        const int key = t * BN + 16 * wave;
         const uint64_t in = __ballot((unsigned)pg_next < (unsigned)a.n_pages);
         const uint64_t none = __ballot(t * BN + 16 * lane >= ext);
-        okay = (uint32_t)(in | none);
-        bad_page |= (okay & ((1u << NB) - 1)) != (1u << NB) - 1;
-        const bool here = in >> blk & 1;
-        const int pg = here ? __builtin_amdgcn_readlane(pg_next, blk) : 0;
+        okay = (uint32_t)(in | none) & ALL;
+        bad_page |= okay != ALL;
+        const bool here = in >> wave & 1;
+        const int pg = here ? __builtin_amdgcn_readlane(pg_next, wave) : 0;
         toks = here ? min(16, ext - key) : 0;
         off = 2 * (pg * a.page_stride + (key & mask) * a.token_stride);
         if (t + 1 < nt) pg_next = look_up(t + 1);
     };
-    // Every wave loads its quarter.  Tokens that are not there are taken from a place that is (masked below).
+    // Every wave loads its block.  Tokens that are not there are taken from a place that is (masked below).
     auto stage_load = [&](const uint8_t *base, T *lds, bool values) {
 #pragma unroll
         for (int p = 0; p < NL; ++p) {
-            const int key = (wave * NL + p) * RI + lane / (D / 8), ch = lane % (D / 8); // of the tile
-            const int tok = max(0, min(key & 15, toks - 1));
-            lds_load16(base + off, (uint32_t)(tok * ts2 + (ch ^ (values ? 2 * (key & 3) : key & 7)) * 16),
+            const int key = p * RI + lane / (D / 8), ch = lane % (D / 8); // of the block
+            const int t = max(0, min(key, toks - 1));
+            lds_load16(base + off, (uint32_t)(t * ts2 + (ch ^ (values ? 2 * (key & 3) : key & 7)) * 16),
                        lds + (wave * NL + p) * 512);
         }
     };
 
-    f32x16 o[NQ][D / 32];
-    float m[NQ], l[NQ]; // the maximum that weights are taken against, and this lane's sum
+    f32x16 o[D / 32];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) o[n][i] = f32x16{};
-        m[n] = -INFINITY;
-        l[n] = 0.f;
-    }
+    for (int i = 0; i < D / 32; ++i) o[i] = f32x16{};
+    float m = -INFINITY, l = 0.f; // the maximum that weights are taken against, and this lane's sum
     uint32_t ko[4], vo[2];
 #pragma unroll
     for (int i = 0; i < 4; ++i) ko[i] = r * (D * 2) + (((2 * i + h) ^ (r & 7)) * 16);
@@ -219,183 +251,230 @@ __global__ __launch_bounds__(256, NQ * D >= 256 ? 1 : 2) void k_attn_prompt(Attn
         vo[1] = vo[0] ^ 64;
     }
 
-    if (nt > 0) {
-        stage(0);
-        stage_load(kb, s_k[0], false);
-        stage_load(vb, s_v[0], true);
+    if (first_t < nt) {
+        stage(first_t);
+        stage_load(kb, s_k[first_t & 1], false);
+        stage_load(vb, s_v[first_t & 1], true);
     }
     bool fresh = true, part = false;
     uint32_t ok = 0;
-    for (int t = 0; t < nt;) {
+    int first_part = nt; // the first tile that some row does not see all of
+    for (int t = first_t; t < nt;) {
         // Tiles until a row's maximum grows past what its weights allow for; then the outputs are rescaled
         // and the tile's scores computed again.  (Two loops, so that the inner one's outputs are the
         // products' own and stay where those put them.)
-        float mx[NQ];
+        float mx;
         for (;;) {
             const int buf = t & 1;
             const uint8_t *lk = (const uint8_t *)s_k[buf], *lv = (const uint8_t *)s_v[buf];
             if (fresh) {
                 ok = okay;
-                // a tile that some row does not see all of
-                part = (t + 1) * BN > full || (ok & ((1u << NB) - 1)) != (1u << NB) - 1;
+                part = (t + 1) * BN > pl.full || ok != ALL;
                 lds_loaded();
                 __syncthreads(); // tile t is there, and nobody works on tile t - 1
                 // A value that a row does not see meets a weight of 0, which an infinity or NaN would survive:
-                                // in such a tile those are 0 for the products, and the rows that see them get them at the end.
-                                if (part) {
-                                    bool bad = false;
-                #pragma unroll 1
-                                    for (int i = tid; i < BN * D / 8; i += 256) {
-                                        u32x4 *p = (u32x4 *)s_v[buf] + i;
-                                        u32x4 w = *p;
-                                        bool any = false;
-                                        for (int j = 0; j < 4; ++j) any |= not_finite<T>(w[j]);
-                                        if (any) {
-                                            for (int j = 0; j < 4; ++j) w[j] = finite_only<T>(w[j]);
-                                            *p = w;
-                                            bad = true;
-                                        }
-                                    }
-                                    if (bad) s_bad = 1;
-                                    __syncthreads();
-                                }
+                // in such a tile those are 0 for the products, and the rows that see them get them at the end.
+                if (part) {
+                    first_part = min(first_part, t);
+                    bool bad = false;
+#pragma unroll 1
+                    for (int i = tid; i < BN * D / 8; i += 256) {
+                        u32x4 *p = (u32x4 *)s_v[buf] + i;
+                        u32x4 w = *p;
+                        bool any = false;
+                        for (int j = 0; j < 4; ++j) any |= not_finite<T>(w[j]);
+                        if (any) {
+                            for (int j = 0; j < 4; ++j) w[j] = finite_only<T>(w[j]);
+                            *p = w;
+                            bad = true;
+                        }
+                    }
+                    if (bad) s_bad = 1;
+                    __syncthreads();
+                }
                 if (t + 1 < nt) {
                     stage(t + 1);
                     stage_load(kb, s_k[buf ^ 1], false);
                     stage_load(vb, s_v[buf ^ 1], true);
                 }
             }
-            f32x16 s[NQ][NS];
-            auto read_k = [&](int x) { // the score tiles in turn: two chains of sums
-                const int i = x % NS, k = x / NS;
-                return *(const x8 *)(lk + ko[k & 3] + i * (32 * D * 2) + (k >> 2) * 128);
-            };
-            auto mul_k = [&](int x, x8 kf) {
-                const int i = x % NS, k = x / NS;
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) s[n][i] = E::mfma32(kf, qf[n][k], k ? s[n][i] : f32x16{});
-            };
-            products<NS * KS, DEPTH, x8>(read_k, mul_k);
+            f32x16 s[NS];
+            products<NS * KS, DEPTH, x8>(
+                [&](int x) { // the score tiles in turn: two chains of sums
+                    const int i = x % NS, k = x / NS;
+                    return *(const x8 *)(lk + ko[k & 3] + i * (32 * D * 2) + (k >> 2) * 128);
+                },
+                [&](int x, x8 kf) {
+                    const int i = x % NS, k = x / NS;
+                    s[i] = E::mfma32(kf, qf[k], k ? s[i] : f32x16{});
+                });
             if (part)
 #pragma unroll
-                for (int n = 0; n < NQ; ++n)
-#pragma unroll
-                    for (int i = 0; i < NS; ++i)
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int key = 32 * i + 8 * (j >> 2) + 4 * h + (j & 3);
-                            if (t * BN + key >= seen[n] || !(ok >> (2 * i + (j >> 3)) & 1)) s[n][i][j] = -INFINITY;
-                        }
-            bool grows = false;
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                mx[n] = s[n][0][0];
-#pragma unroll
                 for (int i = 0; i < NS; ++i)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) mx[n] = fmaxf(mx[n], s[n][i][j]);
-                mx[n] = fmaxf(mx[n], __shfl_xor(mx[n], 32)) * scale;
-                grows |= mx[n] > m[n] + LAZY;
-            }
-            fresh = !__any(grows);
-            if (!fresh) break;
-            u32x4 pw[NQ][2 * NS]; // the weights, in P^T's operand layout
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                const float base = base_of(m[n]) - SHIFT;
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < NS; ++i)
-#pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        const float p0 = exp2_(__builtin_fmaf(s[n][i][j], scale, -base));
-                        const float p1 = exp2_(__builtin_fmaf(s[n][i][j + 1], scale, -base));
-                        sum += p0 + p1;
-                        pw[n][2 * i + (j >> 3)][(j & 7) >> 1] = E::pack(p0, p1);
+                    for (int j = 0; j < 16; ++j) {
+                        const int key = 32 * i + 8 * (j >> 2) + 4 * h + (j & 3);
+                        if (t * BN + key >= seen || !(ok >> (2 * i + (j >> 3)) & 1)) s[i][j] = -INFINITY;
                     }
-                l[n] += sum;
-            }
-            auto read_v = [&](int x) {
-                const int k = x / (D / 32), i = x % (D / 32);
-                const uint8_t *p = lv + vo[i & 1] + k * (16 * D * 2) + (i >> 1) * 128;
-                const u32x2 v0 = lds_read_tr(p), v1 = lds_read_tr(p + 8 * D * 2);
-                return __builtin_bit_cast(x8, (u32x4{v0.x, v0.y, v1.x, v1.y}));
-            };
-            auto mul_v = [&](int x, x8 vf) {
-                const int k = x / (D / 32), i = x % (D / 32);
+            mx = s[0][0];
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) o[n][i] = E::mfma32(vf, __builtin_bit_cast(x8, pw[n][k]), o[n][i]);
-            };
-            products<NS * D / 16, DEPTH, x8>(read_v, mul_v);
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[i][j]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32)) * scale;
+            if (t == first_t) m = fmaxf(m, mx); // nothing to rescale yet
+            fresh = !__any(mx > m + LAZY);
+            if (!fresh) break;
+            const float base = base_of(m) - SHIFT<T>;
+            float sum = 0.f;
+            u32x4 pw[2 * NS]; // the weights, in P^T's operand layout
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; j += 2) {
+                    const float p0 = exp2_(__builtin_fmaf(s[i][j], scale, -base));
+                    const float p1 = exp2_(__builtin_fmaf(s[i][j + 1], scale, -base));
+                    sum += p0 + p1;
+                    pw[2 * i + (j >> 3)][(j & 7) >> 1] = E::pack(p0, p1);
+                }
+            l += sum;
+            products<NS * D / 16, DEPTH, x8>(
+                [&](int x) {
+                    const int k = x / (D / 32), i = x % (D / 32);
+                    const uint8_t *p = lv + vo[i & 1] + k * (16 * D * 2) + (i >> 1) * 128;
+                    const u32x2 v0 = lds_read_tr(p), v1 = lds_read_tr(p + 8 * D * 2);
+                    return __builtin_bit_cast(x8, (u32x4{v0.x, v0.y, v1.x, v1.y}));
+                },
+                [&](int x, x8 vf) {
+                    const int k = x / (D / 32), i = x % (D / 32);
+                    o[i] = E::mfma32(vf, __builtin_bit_cast(x8, pw[k]), o[i]);
+                });
             if (++t == nt) break;
         }
-        if (t < nt)
+        if (t < nt) {
+            const float mn = fmaxf(m, mx);
+            const float alpha = exp2_(m - base_of(mn));
+            m = mn;
+            l *= alpha;
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                const float mn = fmaxf(m[n], mx[n]);
-                const float alpha = exp2_(m[n] - base_of(mn));
-                m[n] = mn;
-                l[n] *= alpha;
-#pragma unroll
-                for (int i = 0; i < D / 32; ++i) o[n][i] *= alpha;
-            }
+            for (int i = 0; i < D / 32; ++i) o[i] *= alpha;
+        }
     }
     if (bad_page && lane == 0) raise(a.flags, MOE_DEVFLAG_BAD_PAGE);
 
     // ---- the infinities and NaN that were 0 for the products, token by token
     __syncthreads();
     if (*(volatile int *)&s_bad)
-#pragma unroll
-        for (int n = 0; n < NQ; ++n)
 #pragma unroll 1
-            for (int key = full / BN * BN; key < seen[n]; ++key) {
-                const int pg = pages[key >> a.page_shift];
-                if ((unsigned)pg >= (unsigned)a.n_pages) continue;
-                const uint8_t *v = vb + 2 * (pg * a.page_stride + (key & mask) * a.token_stride) + 8 * h;
+        for (int key = first_part * BN; key < min(seen, nt * BN); ++key) {
+            const int pg = pages[key >> a.page_shift];
+            if ((unsigned)pg >= (unsigned)a.n_pages) continue;
+            const uint8_t *v = vb + 2 * (pg * a.page_stride + (key & mask) * a.token_stride) + 8 * h;
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i)
+            for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const u32x2 w = ldg<u32x2>(v + 64 * i + 16 * j);
+                for (int j = 0; j < 4; ++j) {
+                    const u32x2 w = ldg<u32x2>(v + 64 * i + 16 * j);
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const uint32_t e = x & 1 ? w[x >> 1] >> 16 : w[x >> 1] & 0xffffu;
-                            if (not_finite<T>(e)) o[n][i][4 * j + x] += (float)__builtin_bit_cast(T, (uint16_t)e);
-                        }
+                    for (int x = 0; x < 4; ++x) {
+                        const uint32_t e = x & 1 ? w[x >> 1] >> 16 : w[x >> 1] & 0xffffu;
+                        if (not_finite<T>(e)) o[i][4 * j + x] += (float)__builtin_bit_cast(T, (uint16_t)e);
                     }
-            }
+                }
+        }
 
-    // ---- rows out
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-        const float sum = l[n] + __shfl_xor(l[n], 32);
-        if (pair(n) >= nf) continue;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        T *op = (T *)a.o + q_at(n, a.o_stride) + 4 * h;
+    // ---- rows out, or their part
+    const float sum = l + __shfl_xor(l, 32);
+    if (!valid) return;
+    if (!whole) {
+        const size_t pr = part_row(a, blockIdx.y) + wave * 32 + r;
+        if (h == 0) *(f32x2 *)(a.part_ml + 2 * pr) = f32x2{m, sum};
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-                u32x2 w = {E::pack(o[n][i][j] * inv, o[n][i][j + 1] * inv),
-                           E::pack(o[n][i][j + 2] * inv, o[n][i][j + 3] * inv)};
-                if (sum == 0.f) w = u32x2{0u, 0u};
-                *(u32x2 *)(op + 32 * i + 2 * j) = w;
-            }
-        if (a.lse && h == 0)
-            a.lse[q_at(n, a.hq * D) / D] =
-                sum == 0.f ? -INFINITY : (base_of(m[n]) - SHIFT + __log2f(sum)) * 0.69314718055994531f;
+            for (int j = 0; j < 16; j += 4)
+                *(f32x4 *)(a.part + pr * D + 4 * h + 32 * i + 2 * j) =
+                    f32x4{o[i][j], o[i][j + 1], o[i][j + 2], o[i][j + 3]};
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)
+            put_row<T>(a, row, head, D, 4 * h + 32 * i + 2 * j, f32x4{o[i][j], o[i][j + 1], o[i][j + 2], o[i][j + 3]}, m,
+                       sum, SHIFT<T>);
+}
+
+// The partial rows of places that were cut into pieces, JOIN_ROWS a workgroup: sum_p f_p x_p / sum_p f_p l_p,
+// f_p = 2^(m_p - max m), in the pieces' order.
+constexpr int JOIN_ROWS = 8, JOIN_B = 8;
+template <typename T, int D>
+__global__ __launch_bounds__(256) void k_attn_prompt_join(AttnArgs a) {
+    constexpr int TPR = D / 4;
+    const int tid = threadIdx.x;
+    Place pl;
+    if (!find_place(a, tid & 63, D < 256, false, pl)) return;
+    const int tiles = (pl.ext + BN - 1) / BN, n = (tiles + pl.chunk - 1) / pl.chunk;
+    if (n < 2) return;
+    for (int i = tid; i < JOIN_ROWS * TPR; i += 256) {
+        const int r = blockIdx.y * JOIN_ROWS + i / TPR, d = i % TPR * 4;
+        const int64_t pair = pl.f0 + r;
+        if (pair >= pl.nf) continue;
+        const int tok = (int)(pair / a.group), head = pl.hk * a.group + (int)(pair - (int64_t)tok * a.group);
+        float M = -INFINITY, L = 0.f;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < n; p += JOIN_B) {
+            f32x2 ml[JOIN_B];
+            f32x4 v[JOIN_B];
+#pragma unroll
+            for (int j = 0; j < JOIN_B; ++j) {
+                ml[j] = p + j < n ? ldg<f32x2>(a.part_ml + 2 * (part_row(a, p + j) + r)) : f32x2{-INFINITY, 0.f};
+                v[j] = p + j < n ? ldg<f32x4>(a.part + (part_row(a, p + j) + r) * D + d) : f32x4{};
+            }
+            float mn = M;
+#pragma unroll
+            for (int j = 0; j < JOIN_B; ++j) mn = fmaxf(mn, ml[j].x);
+            const float f = exp2_(M - base_of(mn));
+            M = mn;
+            L *= f;
+            x *= f;
+#pragma unroll
+            for (int j = 0; j < JOIN_B; ++j) {
+                const float g = exp2_(ml[j].x - base_of(M));
+                L += g * ml[j].y;
+                x += g * v[j];
+            }
+        }
+        put_row<T>(a, pl.r0 + tok, head, D, d, x, M, L, SHIFT<T>);
+    }
+}
+
+template <typename T, int D>
+hipError_t prompt_d(const AttnArgs &args, hipStream_t st) {
+    AttnArgs a = args;
+    // tiles of the rows however they are divided: each sequence's last one may be short
+    const int64_t places = ((int64_t)a.n_rows * a.group / PR_ROWS + a.n_seqs) * a.hkv;
+    // A quarter of the card's workgroup slots or less: the longest rows are cut into pieces, as many as
+    // fill them once.  64 rows of 16 heads of 256 over 32k tokens: 1144 -> 78 us (99 us cut to fill them
+    // twice), 256 rows over 16k 583 -> 109 us.  With more places the partial rows cost what the pieces
+    // gain: a prompt of 1024 rows of 32/8 heads of 128 (half the slots) 32 us whole, 44 us cut in two.
+    const int64_t slots = (int64_t)a.n_cu * (D == 256 ? 1 : 2), cap = (int64_t)a.max_pages << a.page_shift;
+    const int64_t useful = (cap + BN * PR_MIN_CHUNK - 1) / (BN * PR_MIN_CHUNK);
+    a.splits = 1;
+    if (4 * places <= slots) {
+        int64_t n = slots / places;
+        if (n > useful) n = useful;
+        if (n > PR_MAX_SPLITS) n = PR_MAX_SPLITS;
+        if (n * places * PR_ROWS <= a.part_rows) a.splits = (int)n;
+    }
+    k_attn_prompt<T, D><<<dim3((unsigned)places, a.splits), 256, 0, st>>>(a);
+    if (a.splits > 1) k_attn_prompt_join<T, D><<<dim3((unsigned)places, PR_ROWS / JOIN_ROWS), 256, 0, st>>>(a);
+    return hipGetLastError();
 }
 
 template <typename T>
 hipError_t prompt_t(const AttnArgs &a, int d, hipStream_t st) {
-    // tiles of the rows however they are divided: each sequence's last one may be short
-    const int64_t tiles = (int64_t)a.n_rows * a.group / 128 + a.n_seqs;
-    const unsigned grid = (unsigned)(tiles * a.hkv);
-    if (d == 64) k_attn_prompt<T, 64, 1, 64><<<grid, 256, 0, st>>>(a);
-    else if (d == 128) k_attn_prompt<T, 128, 1, 64><<<grid, 256, 0, st>>>(a);
-    else k_attn_prompt<T, 256, 1, 64><<<grid, 256, 0, st>>>(a);
-    return hipGetLastError();
+    return d == 64 ? prompt_d<T, 64>(a, st) : d == 128 ? prompt_d<T, 128>(a, st) : prompt_d<T, 256>(a, st);
 }
 
 } // namespace
