@@ -176,7 +176,7 @@ moe_status moe_attn_create(int device, const moe_attn_config *cfg, moe_attn **ou
     a->n_cu = ncu;
     a->n_wg = 2 * ncu < DEC_MAX_WG ? 2 * ncu : DEC_MAX_WG;
     // decode: two slots a workgroup; prompt: 3.5 pieces for each place on the card at most (prompt_d)
-    const int64_t dec_rows = (int64_t)a->n_wg * 2 * DEC_WAVES * DEC_HEADS;
+    const int64_t dec_rows = (int64_t)a->n_wg * 2 * DEC_HEADS;
     const int64_t prompt_rows = (int64_t)ncu * (g.head_dim == 256 ? 1 : 2) * 7 / 2 * PR_ROWS;
     a->part_rows = dec_rows > prompt_rows ? dec_rows : prompt_rows;
     struct Part {

@@ -8,10 +8,10 @@
 
 namespace moe {
 
-// A group of rows that several workgroups computed a piece of: rows of sequence b, head group sg, the
-// pieces n of workgroups w0 and on (n < 2: nothing to join).
+// A decode unit and its pieces: sequence b, head block hb, n pieces of workgroups w0 and on (n < 2: nothing
+// to join).
 struct Piece {
-    int b, sg, w0, n;
+    int b, hb, w0, n;
 };
 
 // One call's sequences, cache and rows (see moe_seq_batch and moe_kv_cache for the layout).
@@ -32,10 +32,9 @@ struct AttnArgs {
     float scale_log2;         // scale * log2(e): exponentials are taken in base 2
     float *part;              // workspace: partial rows of pieces (see k_attn_decode.hip)
     float *part_ml;           // ... and each partial row's running maximum and sum
-    Piece *piece;             // ... and the groups to join
+    Piece *piece;             // ... and the units to join
     int n_wg;                 // workgroups of a decode launch
     int n_cu;
-    int wpu_shift;            // decode: log2 of the waves that share a unit
     int splits;               // prompt: pieces of the longest rows
     int64_t part_rows;        // rows that part and part_ml hold
 };

@@ -5,15 +5,13 @@
 // Bound by reading K and V once (4 bytes of K and V for 4 * group operations a head element, far
 // below the matrix rate), so all that matters is to keep every CU's loads in flight:
 //
-//   * A unit is one (sequence, key-value head, up to 16 of its query heads).  Each wave of a
-//     workgroup takes 32 tokens of a unit at a step; `wpu` waves share a unit, so a workgroup has
-//     U = 4 / wpu units of one sequence at work (a group).  wpu = 4 splits a unit the widest;
-//     wpu = 1 leaves nothing to join between waves and has the longest runs.
-//   * Work is cut by the lengths as they are in device memory, not by the host's bound: the groups'
+//   * A unit is one (sequence, key-value head, up to 16 of its query heads), a step of it
+//     DEC_STEP tokens, 32 for each wave of a workgroup.
+//   * Work is cut by the lengths as they are in device memory, not by the host's bound: the units'
 //     steps are numbered through and each of the n_wg resident workgroups takes an equal run of
-//     them.  A run that ends inside a group leaves partial rows (maximum, sum, unnormalised
+//     them.  A run that ends inside a unit leaves partial rows (maximum, sum, unnormalised
 //     output), which a second launch joins in their order (same bits every time).
-//   * A wave works by itself, no barrier until the run leaves the group:
+//   * A wave works by itself, no barrier until the run leaves the unit:
 //       S^T[token][head] = K Q^T       16x16x32 products, A rows = tokens straight from memory
 //                                      (a lane's 16 bytes = 8 elements of one token)
 //       O^T[d][head] += V^T P^T        B = P^T is S^T's own register layout: lane (head, g) holds
@@ -23,17 +21,18 @@
 //     lanes) and swaps them in registers, two v_perm a dword pair; the matrix row m of product j
 //     is element 8 m + j, which only the output's addressing sees.
 //   * A wave's loads of the next 32 tokens' K are issued before the softmax, those of V after the
-//     products: some 16 KB a wave are always under way.
+//     products.
 #include "attn_device.hpp"
 
 namespace moe {
 
 namespace {
 
-// Steps of a sequence's group: one at least, so that an empty one's rows are written too.
-__device__ __forceinline__ int seq_steps(const AttnArgs &a, int b, int cap, int shift) {
-    const int n = min(max(a.kv_len[b], 0), cap);
-    return max(1, (n + (1 << shift) - 1) >> shift);
+constexpr int DEC_STEP = DEC_WAVES * DEC_WAVE_TOK;
+
+// Steps of a sequence's units: one at least, so that an empty one's rows are written too.
+__device__ __forceinline__ int seq_steps(const AttnArgs &a, int b, int cap) {
+    return max(1, (min(max(a.kv_len[b], 0), cap) + DEC_STEP - 1) / DEC_STEP);
 }
 
 // A partial row's maximum and sum: those of a row place lie together, so that a wave loads many
@@ -52,20 +51,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
     constexpr int VS = D / (16 * VW);        // loads a token
     typedef uint32_t vload __attribute__((ext_vector_type(VW / 2)));
     // the waves' rows, 4 floats apart so that 16 lanes' rows start in different banks
-    constexpr int OS = D + 4;
-    constexpr int ROWS = DEC_WAVES * DEC_HEADS; // row places of a group
-    __shared__ float s_o[DEC_WAVES][DEC_HEADS][OS];
+    __shared__ float s_o[DEC_WAVES][DEC_HEADS][D + 4];
     __shared__ f32x2 s_ml[DEC_WAVES][DEC_HEADS];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int c = lane & 15, g = lane >> 4;
     const int cap = a.max_pages << a.page_shift;
     const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS; // head blocks of a key-value head
-    const int wpu = 1 << a.wpu_shift, U = DEC_WAVES >> a.wpu_shift;
-    const int shift = 5 + a.wpu_shift;                    // log2 of a step's tokens
-    const int ng = a.hkv * gb / U;                        // groups of a sequence
-    const int sub = wave >> a.wpu_shift, wsub = wave & (wpu - 1);
-    const int rows = min(DEC_HEADS, a.group);             // row places of a unit
+    const int ng = a.hkv * gb;                            // units of a sequence
 
     // ---- this workgroup's run of steps [lo, hi): every wave sums the sequences' steps by itself,
     // a lane those of `per` in a row, and finds the sequence that lo lies in
@@ -73,63 +66,52 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
     uint32_t mine = 0;
     for (int i = 0; i < per; ++i) {
         const int b = lane * per + i;
-        if (b < a.n_seqs) mine += (uint32_t)seq_steps(a, b, cap, shift);
+        if (b < a.n_seqs) mine += (uint32_t)seq_steps(a, b, cap);
     }
     const uint32_t incl = wave_scan(mine);
     const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63) * ng;
     const uint32_t share = (total + gridDim.x - 1) / gridDim.x;
     const uint32_t lo = blockIdx.x * share;
+    // For the join: of every unit the pieces it was cut into, or (more units than workgroups) of every
+    // workgroup those of the unit that it begins and others go on with.
+    const bool by_unit = (int64_t)a.n_seqs * ng <= a.n_wg;
+    Piece tail = {0, 0, 0, 0};
     if (lo >= total) {
-        if (tid == 0 && (int64_t)a.n_seqs * ng > a.n_wg) a.piece[blockIdx.x] = Piece{0, 0, 0, 0};
+        if (!by_unit && tid == 0) a.piece[blockIdx.x] = tail;
         return;
     }
     const uint32_t hi = min(lo + share, total);
     const int owner = __builtin_ctzll(__ballot(incl * ng > lo));
-    uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), owner); // steps before b, of one group
-    int b = owner * per, nt = uniform(seq_steps(a, b, cap, shift));
+    uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), owner); // steps before b, of one unit each
+    int b = owner * per, nt = uniform(seq_steps(a, b, cap));
     while ((at + nt) * ng <= lo) {
         at += nt;
-        nt = uniform(seq_steps(a, ++b, cap, shift));
+        nt = uniform(seq_steps(a, ++b, cap));
     }
-    int sg = (int)((lo - at * ng) / (uint32_t)nt);
-    uint32_t unit = at * ng + sg * nt; // first step of group (b, sg)
+    int hb = (int)((lo - at * ng) / (uint32_t)nt);
+    uint32_t unit = at * ng + hb * nt; // first step of unit (b, hb)
 
-    // a unit's key-value head, first query head and heads
+    // a unit's first query head and heads
     auto head0 = [&](int hb) { return hb / gb * a.group + hb % gb * DEC_HEADS; };
     auto heads = [&](int hb) { return min(DEC_HEADS, a.group - hb % gb * DEC_HEADS); };
-    const int items = U * rows * (D / 4);
-    // For the join: of every group the pieces it was cut into, or (more groups than workgroups) of every
-    // workgroup those of the group that it begins and others go on with.
-    const bool by_group = (int64_t)a.n_seqs * ng <= a.n_wg;
-    Piece tail = {0, 0, 0, 0};
 
-    for (uint32_t pos = lo; pos < hi;) {
-        const int t0 = (int)(pos - unit);
-        const int t1 = (int)((hi < unit + nt ? hi : unit + nt) - unit);
-        const int len = ldc(a.kv_len + b);
-        const int seen = min(max(len, 0), cap);
+    const int ts2 = (int)(2 * a.token_stride), mask = (1 << a.page_shift) - 1;
+    bool bad = false;
+    for (uint32_t pos = lo;;) {
+        // ---- the unit at work: steps t0..t1 of it
+        const int t0 = (int)(pos - unit), t1 = (int)(min(hi, unit + nt) - unit);
+        const int len = ldc(a.kv_len + b), seen = min(max(len, 0), cap);
         if (seen != len && tid == 0) raise(a.flags, MOE_DEVFLAG_BAD_SEQ);
-        const int hb = sg * U + sub, hk = hb / gb;
-        const T *q = (const T *)a.q + b * a.q_stride + (int64_t)(head0(hb) + min(c, heads(hb) - 1)) * D;
-        // The queries' fragments stay in registers; at D = 256, where those are short, in the wave's own
-        // part of s_o, every lane reading back what it wrote.
-        x8 qf[KS];
-#pragma unroll
-        for (int k = 0; k < KS; ++k) qf[k] = ldg<x8>(q + k * 32 + g * 8);
-
-        f32x4 acc[D / 16];
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float m = -INFINITY, l = 0.f;
+        const int end = min(seen, t1 * DEC_STEP); // of the tokens
+        const int hk = hb / gb, nh = heads(hb);
         const int32_t *pages = a.pages + b * a.pages_stride;
         const uint8_t *kb = a.k + 2 * hk * a.head_stride, *vb = a.v + 2 * hk * a.head_stride;
-        const int ts2 = (int)(2 * a.token_stride);
-        const int mask = (1 << a.page_shift) - 1;
-        const int end = min(seen, t1 << shift); // of this piece
-        bool bad = false;
-
-        // the two 16-token halves of a step: byte offset of the first token, tokens there
-        int64_t off[2];
+        const T *q = (const T *)a.q + b * a.q_stride + (int64_t)(head0(hb) + min(c, nh - 1)) * D;
+        x8 qf[KS], kf[2][KS];
+        vload vf[8][VS];
+#pragma unroll
+        for (int k = 0; k < KS; ++k) qf[k] = ldg<x8>(q + k * 32 + g * 8);
+        int64_t off[2]; // the two 16-token halves of a step: byte offset of the first token, tokens there
         int have[2];
         auto place = [&](int tok) {
 #pragma unroll
@@ -144,8 +126,6 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
                 off[i] = 2 * (pg * a.page_stride + (t & mask) * a.token_stride);
             }
         };
-        x8 kf[2][KS];
-        vload vf[8][VS];
         // a lane whose token is not there reads the last one that is (the first place if none is)
         auto lane_off = [&](int t, int i, int byte) {
             if (have[i] < 16) t = max(0, min(t, have[i] - 1));
@@ -162,24 +142,28 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
         auto load_v = [&]() {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int i = j >> 2;
-                const uint32_t lo = lane_off(4 * g + (j & 3), i, c * (VW * 2));
+                const uint32_t lo = lane_off(4 * g + (j & 3), j >> 2, c * (VW * 2));
 #pragma unroll
-                for (int s = 0; s < VS; ++s) vf[j][s] = ldo<vload>(vb + off[i], lo, s * (32 * VW));
+                for (int s = 0; s < VS; ++s) vf[j][s] = ldo<vload>(vb + off[j >> 2], lo, s * (32 * VW));
             }
         };
-        int tok = (t0 << shift) + wsub * DEC_WAVE_TOK;
-        const int step = 1 << shift;
+        int tok = t0 * DEC_STEP + wave * DEC_WAVE_TOK;
         if (tok < end) {
             place(tok);
             load_k();
             load_v();
         }
+        // The queries' fragments stay in registers; at D = 256, where those are short, in the wave's own
+        // part of s_o, every lane reading back what it wrote.
         x8 *const ql = (x8 *)&s_o[wave][0][0] + lane;
         if (D == 256)
 #pragma unroll
             for (int k = 0; k < KS; ++k) ql[64 * k] = qf[k];
-        for (; tok < end; tok += step) {
+        f32x4 acc[D / 16];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+        for (; tok < end; tok += DEC_STEP) {
             const int hv[2] = {have[0], have[1]};
             f32x4 st[2];
 #pragma unroll
@@ -190,9 +174,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
                 for (int i = 0; i < 2; ++i)
                     st[i] = E::mfma16(kf[i][k], qk, k ? st[i] : f32x4{0.f, 0.f, 0.f, 0.f});
             }
-            const bool more = tok + step < end;
+            const bool more = tok + DEC_STEP < end;
             if (more) {
-                place(tok + step);
+                place(tok + DEC_STEP);
                 load_k();
             }
             float mx = m;
@@ -239,7 +223,6 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
                 }
             if (more) load_v();
         }
-        if (bad && lane == 0) raise(a.flags, MOE_DEVFLAG_BAD_PAGE);
 
         // ---- join the four waves: row (head c) of O^T's register layout to s_o[wave][head][d]
         l += __shfl_xor(l, 16);
@@ -254,62 +237,60 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
                 for (int j = 0; j < VW; j += 4)
                     *(f32x4 *)&s_o[wave][c][16 * VW * s + VW * (4 * g + r) + j] =
                         f32x4{acc[s * VW + j][r], acc[s * VW + j + 1][r], acc[s * VW + j + 2][r], acc[s * VW + j + 3][r]};
-        __syncthreads();
-        const bool whole = t0 == 0 && t1 == nt;
+        const bool begins = t0 == 0, whole = begins && t1 == nt;
+        const Piece pc = {b, hb, (int)blockIdx.x, (int)((unit + nt - 1) / share - blockIdx.x + 1)};
+        lds_barrier();
+        // Partial rows: slot 0 of a workgroup holds the piece of a unit that began before it, slot 1 that
+        // of one which goes on behind it.
+        const size_t slot = 2 * (size_t)blockIdx.x + (begins ? 1 : 0);
         int et = tid; // opaque, so that no item's index is computed before the loop and held through it
         asm volatile("" : "+v"(et));
-        // Partial rows: slot 0 of a workgroup holds the piece of a group that began before it, slot 1
-        // that of one which goes on behind it.
-        const size_t slot = 2 * (size_t)blockIdx.x + (t0 == 0 ? 1 : 0);
-        for (int i = et; i < items; i += 256) {
-            const int r = i / (D / 4), d = i % (D / 4) * 4, u = r / rows, hh = r % rows;
-            if (hh >= heads(sg * U + u)) continue;
-            const int w0 = u << a.wpu_shift;
-            f32x2 ml[DEC_WAVES];
-            f32x4 y[DEC_WAVES];
+        {
+            const auto &a = fresh_args();
+            for (int i = et; i < nh * (D / 4); i += 256) {
+                const int hh = i / (D / 4), d = i % (D / 4) * 4;
+                f32x2 ml[DEC_WAVES];
+                f32x4 y[DEC_WAVES], x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < DEC_WAVES; ++w) { // fewer waves: some twice, the second time as nothing
-                ml[w] = s_ml[w0 + (w & (wpu - 1))][hh];
-                y[w] = *(const f32x4 *)&s_o[w0 + (w & (wpu - 1))][hh][d];
-            }
-            float M = -INFINITY, L = 0.f;
+                for (int w = 0; w < DEC_WAVES; ++w) {
+                    ml[w] = s_ml[w][hh];
+                    y[w] = *(const f32x4 *)&s_o[w][hh][d];
+                }
+                float M = -INFINITY, L = 0.f;
 #pragma unroll
-            for (int w = 0; w < DEC_WAVES; ++w) M = fmaxf(M, ml[w].x);
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                for (int w = 0; w < DEC_WAVES; ++w) M = fmaxf(M, ml[w].x);
 #pragma unroll
-            for (int w = 0; w < DEC_WAVES; ++w)
-                if (w < wpu) {
+                for (int w = 0; w < DEC_WAVES; ++w) {
                     const float f = exp2_(ml[w].x - base_of(M));
                     L += f * ml[w].y;
                     x += f * y[w];
                 }
-            if (whole) put_row<T>(a, b, head0(sg * U + u) + hh, D, d, x, M, L, E::SHIFT);
-            else {
-                *(f32x4 *)(a.part + (slot * ROWS + u * DEC_HEADS + hh) * D + d) = x;
-                if (d == 0) *(f32x2 *)(a.part_ml + ml_at(a, u * DEC_HEADS + hh, slot)) = f32x2{M, L};
+                if (whole) put_row<T>(a, b, head0(hb) + hh, D, d, x, M, L, E::SHIFT);
+                else {
+                    *(f32x4 *)(a.part + (slot * DEC_HEADS + hh) * D + d) = x;
+                    if (d == 0) *(f32x2 *)(a.part_ml + ml_at(a, hh, slot)) = f32x2{M, L};
+                }
             }
-        }
-        if (t0 == 0) {
-            const Piece pc = {b, sg, (int)blockIdx.x, (int)((unit + nt - 1) / share - blockIdx.x + 1)};
-            if (by_group) {
-                if (tid == 0) a.piece[b * ng + sg] = pc;
-            } else if (!whole) tail = pc;
+            if (begins) {
+                if (by_unit) {
+                    if (tid == 0) a.piece[b * ng + hb] = pc;
+                } else if (!whole) tail = pc;
+            }
         }
         pos = unit + t1;
-        if (pos < hi) { // the next (sequence, heads)
-            __syncthreads(); // s_o is free again
-            unit += nt;
-            if (++sg == ng) {
-                sg = 0;
-                ++b;
-                nt = uniform(seq_steps(a, b, cap, shift));
-            }
+        if (pos >= hi) break;
+        lds_barrier(); // s_o is free again
+        unit += nt; // the next unit
+        if (++hb == ng) {
+            hb = 0;
+            nt = uniform(seq_steps(a, ++b, cap));
         }
     }
-    if (!by_group && tid == 0) a.piece[blockIdx.x] = tail;
+    if (bad && lane == 0) raise(a.flags, MOE_DEVFLAG_BAD_PAGE);
+    if (!by_unit && tid == 0) a.piece[blockIdx.x] = tail;
 }
 
-// The partial rows of a group that several runs share: out = sum_p f_p x_p / sum_p f_p l_p,
+// The partial rows of a unit that several runs share: out = sum_p f_p x_p / sum_p f_p l_p,
 // f_p = 2^(m_p - max m), in the pieces' order.  Up to JOIN_FEW pieces: a thread takes four elements of a
 // row through all of them.  More: a row at a time, a thread four elements of every PG-th piece, JOIN_B of
 // them under way.
@@ -319,32 +300,26 @@ __global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_
     constexpr int TPR = D / 4, PG = THREADS / TPR;
     __shared__ float s_f[DEC_MAX_WG];
     __shared__ f32x4 s_x[PG][TPR];
-    const Piece pc = {ldc(&a.piece[blockIdx.x].b), ldc(&a.piece[blockIdx.x].sg), ldc(&a.piece[blockIdx.x].w0),
+    const Piece pc = {ldc(&a.piece[blockIdx.x].b), ldc(&a.piece[blockIdx.x].hb), ldc(&a.piece[blockIdx.x].w0),
                       ldc(&a.piece[blockIdx.x].n)};
     const int n = pc.n;
     if (n < 2) return;
     const int tid = threadIdx.x, lane = tid & 63;
-    const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS, U = DEC_WAVES >> a.wpu_shift;
-    const int rows = min(DEC_HEADS, a.group);
-    const int r0 = blockIdx.y * rows_per_wg, r1 = min(U * rows, r0 + rows_per_wg);
+    const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS;
+    const int h0 = pc.hb / gb * a.group + pc.hb % gb * DEC_HEADS; // the unit's first query head, and its heads
+    const int nh = min(DEC_HEADS, a.group - pc.hb % gb * DEC_HEADS);
+    const int r0 = blockIdx.y * rows_per_wg, r1 = min(nh, r0 + rows_per_wg);
     // row r of piece p: of the first workgroup the later slot, of the others the earlier one
     auto slot = [&](int p) { return 2 * (size_t)(pc.w0 + p) + (p == 0 ? 1 : 0); };
-    auto place = [&](int r) { return r / rows * DEC_HEADS + r % rows; };
-    auto row = [&](int r, int p) { return slot(p) * (DEC_WAVES * DEC_HEADS) + place(r); };
-    // its query head, or -1 for a place that the last head block does not have
-    auto head = [&](int r) {
-        const int hb = pc.sg * U + r / rows, hh = r % rows;
-        return hh < a.group - hb % gb * DEC_HEADS ? hb / gb * a.group + hb % gb * DEC_HEADS + hh : -1;
-    };
+    auto row = [&](int r, int p) { return slot(p) * DEC_HEADS + r; };
     if (n <= JOIN_FEW) {
         for (int i = r0 * TPR + tid; i < r1 * TPR; i += THREADS) {
-            const int r = i / TPR, d = i % TPR * 4, h = head(r);
-            if (h < 0) continue;
+            const int r = i / TPR, d = i % TPR * 4;
             f32x2 ml[JOIN_FEW];
             f32x4 v[JOIN_FEW];
 #pragma unroll
             for (int p = 0; p < JOIN_FEW; ++p) {
-                ml[p] = p < n ? ldg<f32x2>(a.part_ml + ml_at(a, place(r), slot(p))) : f32x2{-INFINITY, 0.f};
+                ml[p] = p < n ? ldg<f32x2>(a.part_ml + ml_at(a, r, slot(p))) : f32x2{-INFINITY, 0.f};
                 v[p] = p < n ? ldg<f32x4>(a.part + row(r, p) * D + d) : f32x4{};
             }
             float M = -INFINITY, L = 0.f;
@@ -357,14 +332,12 @@ __global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_
                 L += f * ml[p].y;
                 x += f * v[p];
             }
-            put_row<T>(a, pc.b, h, D, d, x, M, L, Elem<T>::SHIFT);
+            put_row<T>(a, pc.b, h0 + r, D, d, x, M, L, Elem<T>::SHIFT);
         }
         return;
     }
     const int pg = tid / TPR, d = tid % TPR * 4;
     for (int r = r0; r < r1; ++r) {
-        const int h = head(r);
-        if (h < 0) continue;
         f32x4 v[JOIN_B];
         auto load = [&](int p) {
 #pragma unroll
@@ -373,10 +346,10 @@ __global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_
         };
         load(pg);
         float M = -INFINITY, L = 0.f;
-        for (int p = lane; p < n; p += 64) M = fmaxf(M, ldg<f32x2>(a.part_ml + ml_at(a, place(r), slot(p))).x);
+        for (int p = lane; p < n; p += 64) M = fmaxf(M, ldg<f32x2>(a.part_ml + ml_at(a, r, slot(p))).x);
         M = wave_max(M);
         for (int p = lane; p < n; p += 64) {
-            const f32x2 ml = ldg<f32x2>(a.part_ml + ml_at(a, place(r), slot(p)));
+            const f32x2 ml = ldg<f32x2>(a.part_ml + ml_at(a, r, slot(p)));
             const float f = exp2_(ml.x - base_of(M));
             L += f * ml.y;
             if (tid < 64) s_f[p] = f;
@@ -395,7 +368,7 @@ __global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_
         lds_barrier();
         if (pg == 0) {
             for (int i = 1; i < PG; ++i) x += s_x[i][tid];
-            put_row<T>(a, pc.b, h, D, d, x, M, L, Elem<T>::SHIFT);
+            put_row<T>(a, pc.b, h0 + r, D, d, x, M, L, Elem<T>::SHIFT);
         }
         lds_barrier(); // s_f and s_x are free again
     }
@@ -404,12 +377,11 @@ __global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_
 template <typename T, int D>
 hipError_t decode_d(const AttnArgs &a, hipStream_t st) {
     k_attn_decode<T, D><<<a.n_wg, 256, 0, st>>>(a);
-    // Few groups, so possibly many pieces each: one row a workgroup of 512.  Many, so two or three
-    // pieces of each mostly: the rows that 256 threads hold.
-    const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS, U = DEC_WAVES >> a.wpu_shift;
-    const int rows = U * (a.group < DEC_HEADS ? a.group : DEC_HEADS);
-    const int64_t groups = (int64_t)a.n_seqs * (a.hkv * gb / U);
-    const int x = groups <= a.n_wg ? (int)groups : a.n_wg, per = 1024 / D;
+    // Few units, so possibly many pieces each: one row a workgroup of 512.  Many, so a few pieces of each
+    // mostly: the rows that 256 threads hold.
+    const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS, rows = a.group < DEC_HEADS ? a.group : DEC_HEADS;
+    const int64_t units = (int64_t)a.n_seqs * a.hkv * gb;
+    const int x = units <= a.n_wg ? (int)units : a.n_wg, per = 1024 / D;
     if (x * rows <= 512) k_attn_join<T, D, 512><<<dim3(x, rows), 512, 0, st>>>(a, 1);
     else if (x * rows <= 2048) k_attn_join<T, D, 256><<<dim3(x, rows), 256, 0, st>>>(a, 1);
     else k_attn_join<T, D, 256><<<dim3(x, (rows + per - 1) / per), 256, 0, st>>>(a, per);
@@ -423,14 +395,7 @@ hipError_t decode_t(const AttnArgs &a, int d, hipStream_t st) {
 
 } // namespace
 
-hipError_t launch_attn_decode(const AttnArgs &args, int type, int d, hipStream_t st) {
-    AttnArgs a = args;
-    // Units enough for every workgroup to have several at once: let fewer waves share one.
-    const int hb = a.hkv * ((a.group + DEC_HEADS - 1) / DEC_HEADS);
-    const int64_t units = (int64_t)a.n_seqs * hb;
-    a.wpu_shift = 2;
-    if (hb % 4 == 0 && units >= 4 * a.n_wg) a.wpu_shift = 0;
-    else if (hb % 2 == 0 && units >= 2 * a.n_wg) a.wpu_shift = 1;
+hipError_t launch_attn_decode(const AttnArgs &a, int type, int d, hipStream_t st) {
     return type == MOE_T_F16 ? decode_t<f16_t>(a, d, st) : decode_t<bf16_t>(a, d, st);
 }
 
