@@ -298,7 +298,7 @@ typedef struct {
  * page_tokens; entries behind the last used page are not read), the number of cached tokens
  * kv_len[b], the new ones included, and its rows row_start[b]..row_start[b+1]-1 of the packed
  * row arrays (row_start ascends; the last row is the last new token).  row_start = NULL: one
- * row a sequence.  n_rows: rows of the packed arrays; those of no sequence (behind the last
+ * row a sequence.  n_rows: rows of the packed arrays, at most 2^22; those of no sequence (behind the last
  * one's, say) are left as they were. */
 typedef struct {
     int n_seqs;

@@ -58,8 +58,8 @@ moe_status common_args(const char *fn, moe_attn *a, const moe_kv_cache *kv, cons
     const moe_attn_config &g = a->cfg;
     if (s->n_seqs < 0 || s->n_seqs > g.max_seqs)
         return fail(MOE_EINVAL, "%s: %d sequences outside 0..max_seqs=%d", fn, s->n_seqs, g.max_seqs);
-    if (s->n_rows < 0 || s->n_rows > (1 << 24))
-        return fail(MOE_EINVAL, "%s: %d rows outside 0..2^24", fn, s->n_rows);
+    if (s->n_rows < 0 || s->n_rows > (1 << 22)) // (rows * heads) are counted in 31 bits
+        return fail(MOE_EINVAL, "%s: %d rows outside 0..2^22", fn, s->n_rows);
     if (!s->row_start && s->n_rows != s->n_seqs)
         return fail(MOE_EINVAL, "%s: %d rows of %d sequences without row_start", fn, s->n_rows, s->n_seqs);
     if (s->max_pages < 1 || s->max_pages > ((1 << 30) >> a->page_shift))

@@ -43,7 +43,7 @@ __device__ __forceinline__ Rows seq_rows(const AttnArgs &a, int b) {
 }
 
 // Tokens that the f-th (token, head) pair's row of a sequence sees, its first row's position given.
-__device__ __forceinline__ int seen_by(const AttnArgs &a, int64_t first_pos, int64_t f) {
+__device__ __forceinline__ int seen_by(const AttnArgs &a, int64_t first_pos, int f) {
     const int64_t p = first_pos + f / a.group + 1, cap = (int64_t)a.max_pages << a.page_shift;
     return (int)(p < 0 ? 0 : p > cap ? cap : p);
 }
@@ -81,7 +81,8 @@ __device__ __forceinline__ void products(Read read, Product product) {
 // last one sees ext tokens and the first one `full`; pieces of them, `chunk` tiles each.
 struct Place {
     int b, r0, hk;
-    int64_t f0, nf, first_pos; // of the sequence's first row
+    int f0, nf;
+    int64_t first_pos; // of the sequence's first row
     int ext, full, chunk;
 };
 
@@ -91,7 +92,7 @@ struct Place {
 __device__ __forceinline__ bool find_place(const AttnArgs &a, int lane, bool snake, bool flag, Place &pl) {
     const int cap = a.max_pages << a.page_shift;
     const int per = (a.n_seqs + 63) / 64;
-    auto tiles = [&](int n) { return (uint32_t)(((int64_t)n * a.group + PR_ROWS - 1) / PR_ROWS); };
+    auto tiles = [&](int n) { return ((uint32_t)n * a.group + PR_ROWS - 1) / PR_ROWS; };
     uint32_t mine = 0;
     int most = 0; // tokens that a row sees
     bool bad = false;
@@ -130,8 +131,8 @@ __device__ __forceinline__ bool find_place(const AttnArgs &a, int lane, bool sna
     pl.b = uniform(b);
     pl.r0 = uniform(sr.r0);
     pl.hk = blockIdx.x - nth * a.hkv;
-    pl.f0 = (int64_t)(want - at) * PR_ROWS;
-    pl.nf = (int64_t)uniform(sr.n) * a.group;
+    pl.f0 = (int)(want - at) * PR_ROWS;
+    pl.nf = uniform(sr.n) * a.group;
     pl.first_pos = (int64_t)ldc(a.kv_len + pl.b) - ldc(a.row_start + pl.b + 1) + pl.r0;
     pl.full = uniform(seen_by(a, pl.first_pos, pl.f0));
     pl.ext = uniform(seen_by(a, pl.first_pos, min(pl.f0 + PR_ROWS, pl.nf) - 1));
@@ -180,22 +181,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
     if (tid == 0) s_bad = 0;
 
     // this lane's row; one behind the last reads the last one's query and sees nothing
-    const int64_t pair = pl.f0 + wave * 32 + r;
+    const int pair = pl.f0 + wave * 32 + r;
     const bool valid = pair < pl.nf;
-    const int tok = (int)((valid ? pair : pl.nf - 1) / a.group);
-    const int row = pl.r0 + tok, head = pl.hk * a.group + (int)((valid ? pair : pl.nf - 1) - (int64_t)tok * a.group);
+    const int tok = min(pair, pl.nf - 1) / a.group;
+    const int row = pl.r0 + tok, head = pl.hk * a.group + min(pair, pl.nf - 1) - tok * a.group;
     const int seen = valid ? seen_by(a, pl.first_pos, pair) : 0;
-    x8 qf[KS];
-    {
-        const T *q = (const T *)a.q + row * a.q_stride + head * D + h * 8;
-        const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u; // a negative scale: -q, exactly
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            u32x4 w = ldg<u32x4>(q + k * 16);
-            for (int i = 0; i < 4; ++i) w[i] ^= flip;
-            qf[k] = __builtin_bit_cast(x8, w);
-        }
-    }
     // Scale 0: the smallest normal number, so that -inf (not seen) stays -inf; any finite score times it
     // is 0 beside the exponential's 1.
     const float scale = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);
@@ -213,6 +203,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
         return lane < NB && key < ext ? ldg<int>(pages + (key >> a.page_shift)) : -1;
     };
     int pg_next = look_up(first_t);
+    u32x4 qw[KS];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qw[k] = ldg<u32x4>((const T *)a.q + row * a.q_stride + head * D + h * 8 + k * 16);
     int64_t off = 0; // of this wave's block of the tile; tokens there
     int toks = 0;
     auto stage = [&](int t) {
@@ -256,6 +249,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
         stage_load(kb, s_k[first_t & 1], false);
         stage_load(vb, s_v[first_t & 1], true);
     }
+    x8 qf[KS];
+    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u; // a negative scale: -q, exactly
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qf[k] = __builtin_bit_cast(x8, qw[k] ^ flip);
     bool fresh = true, part = false;
     uint32_t ok = 0;
     int first_part = nt; // the first tile that some row does not see all of
@@ -276,16 +273,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
                 // in such a tile those are 0 for the products, and the rows that see them get them at the end.
                 if (part) {
                     first_part = min(first_part, t);
+                    constexpr int NW = BN * D / 8 / 256;
+                    u32x4 w[NW];
                     bool bad = false;
-#pragma unroll 1
-                    for (int i = tid; i < BN * D / 8; i += 256) {
-                        u32x4 *p = (u32x4 *)s_v[buf] + i;
-                        u32x4 w = *p;
+#pragma unroll
+                    for (int i = 0; i < NW; ++i) w[i] = ((const u32x4 *)s_v[buf])[tid + 256 * i];
+#pragma unroll
+                    for (int i = 0; i < NW; ++i) {
                         bool any = false;
-                        for (int j = 0; j < 4; ++j) any |= not_finite<T>(w[j]);
+                        for (int j = 0; j < 4; ++j) any |= not_finite<T>(w[i][j]);
                         if (any) {
-                            for (int j = 0; j < 4; ++j) w[j] = finite_only<T>(w[j]);
-                            *p = w;
+                            for (int j = 0; j < 4; ++j) w[i][j] = finite_only<T>(w[i][j]);
+                            ((u32x4 *)s_v[buf])[tid + 256 * i] = w[i];
                             bad = true;
                         }
                     }
@@ -385,8 +384,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
 
     // ---- rows out, or their part
     const float sum = l + __shfl_xor(l, 32);
-    if (!valid) return;
     if (!whole) {
+        if (!valid) return;
         const size_t pr = part_row(a, blockIdx.y) + wave * 32 + r;
         if (h == 0) *(f32x2 *)(a.part_ml + 2 * pr) = f32x2{m, sum};
 #pragma unroll
@@ -397,12 +396,37 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
                     f32x4{o[i][j], o[i][j + 1], o[i][j + 2], o[i][j + 3]};
         return;
     }
+    // Through LDS, so that whole rows are stored: a wave's rows in a part of its own, 16 bytes between them.
+    // (The tiles are done with: the barrier before the infinities.)
+    constexpr int OS = D + 8;
+    static_assert(128 * OS <= 4 * BN * D, "the rows in the tiles' place");
+    T *so = (wave < 2 ? s_k[0] : s_v[0]) + (wave & 1) * 32 * OS;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-        for (int j = 0; j < 16; j += 4)
-            put_row<T>(a, row, head, D, 4 * h + 32 * i + 2 * j, f32x4{o[i][j], o[i][j + 1], o[i][j + 2], o[i][j + 3]}, m,
-                       sum, SHIFT<T>);
+        for (int j = 0; j < 16; j += 4) {
+            u32x2 w = {E::pack(o[i][j] * inv, o[i][j + 1] * inv), E::pack(o[i][j + 2] * inv, o[i][j + 3] * inv)};
+            if (sum == 0.f) w = u32x2{0u, 0u};
+            *(u32x2 *)(so + r * OS + 4 * h + 32 * i + 2 * j) = w;
+        }
+    if (a.lse && valid && h == 0)
+        a.lse[(int64_t)row * a.hq + head] =
+            sum == 0.f ? -INFINITY : (base_of(m) - SHIFT<T> + __log2f(sum)) * 0.69314718055994531f;
+    constexpr int LR = D / 8; // lanes of a row
+    const int f0 = pl.f0 + wave * 32, n = min(32, pl.nf - f0);
+    const int t0 = f0 / a.group, y0 = f0 - t0 * a.group; // the first row's token and head
+    const float by_group = 1.f / (float)a.group;
+#pragma unroll
+    for (int i = 0; i < LR / 2; ++i) { // 64 / LR rows at a time
+        const int x = i * (64 / LR) + lane / LR;
+        const u32x4 w = *(const u32x4 *)(so + x * OS + lane % LR * 8);
+        if (x < n) {
+            // (y0 + x) / group, below 256 + 32: exact in f32
+            const int t = (int)(((float)(y0 + x) + 0.5f) * by_group), hd = pl.hk * a.group + y0 + x - t * a.group;
+            *(u32x4 *)((T *)a.o + (pl.r0 + t0 + t) * a.o_stride + hd * D + lane % LR * 8) = w;
+        }
+    }
 }
 
 // The partial rows of places that were cut into pieces, JOIN_ROWS a workgroup: sum_p f_p x_p / sum_p f_p l_p,
@@ -418,9 +442,9 @@ __global__ __launch_bounds__(256) void k_attn_prompt_join(AttnArgs a) {
     if (n < 2) return;
     for (int i = tid; i < JOIN_ROWS * TPR; i += 256) {
         const int r = blockIdx.y * JOIN_ROWS + i / TPR, d = i % TPR * 4;
-        const int64_t pair = pl.f0 + r;
+        const int pair = pl.f0 + r;
         if (pair >= pl.nf) continue;
-        const int tok = (int)(pair / a.group), head = pl.hk * a.group + (int)(pair - (int64_t)tok * a.group);
+        const int tok = pair / a.group, head = pl.hk * a.group + pair - tok * a.group;
         float M = -INFINITY, L = 0.f;
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
         for (int p = 0; p < n; p += JOIN_B) {
