@@ -266,8 +266,9 @@ moe_status moe_stack_trace(moe_ctx *ctx, uint64_t *buf, size_t words);
  *
  * A moe_attn holds one layer shape and its workspaces, as a moe_ctx does: one stream/thread
  * at a time (graphs captured from one moe_attn share its workspaces: replay them in order on
- * one stream, or capture them from handles of their own), no allocation after creation.  A
- * call runs on the handle's device whatever the current one is; `stream` belongs to it. */
+ * one stream, or capture them from handles of their own), no allocation after creation (about
+ * 34 MB of device memory at most).  A call runs on the handle's device whatever the current one
+ * is; `stream` belongs to it. */
 typedef struct moe_attn moe_attn;
 
 /* Element types, by their GGML type ids. */
@@ -286,7 +287,8 @@ typedef struct {
 /* A cache: element (page, head, token, i) of the keys at
  *   k + page * page_stride + head * head_stride + token * token_stride + i   (elements),
  * the values with the same strides from v.  Any order of page, head and token; strides are
- * positive multiples of 8 elements, k and v 16-byte aligned, i contiguous. */
+ * multiples of 8 elements and head_dim at least, token_stride 2^24 at most, k and v 16-byte
+ * aligned, i contiguous. */
 typedef struct {
     void *k, *v;
     int n_pages;
@@ -298,8 +300,9 @@ typedef struct {
  * page_tokens; entries behind the last used page are not read), the number of cached tokens
  * kv_len[b], the new ones included, and its rows row_start[b]..row_start[b+1]-1 of the packed
  * row arrays (row_start ascends; the last row is the last new token).  row_start = NULL: one
- * row a sequence.  n_rows: rows of the packed arrays, at most 2^22; those of no sequence (behind the last
- * one's, say) are left as they were. */
+ * row a sequence.  n_rows: rows of the packed arrays, at most 2^22; those of no sequence (behind
+ * the last one's, say) are left as they were.  A page list holds 2^30 tokens at most, and (its
+ * tokens + 32) x n_seqs x n_kv_heads (x head blocks of 16 of a group of more) stay below 2^36. */
 typedef struct {
     int n_seqs;
     int n_rows;
@@ -319,8 +322,8 @@ moe_status moe_attn_destroy(moe_attn *a);
  * k_row_stride / v_row_stride elements apart (a slice of a fused projection's rows: multiples of 16
  * bytes; 16-byte aligned), to the places kv_len[b] - n_b .. kv_len[b] - 1 of their sequences.
  * in_type: the cache's type, or MOE_T_F32 (rounded to nearest even).  Tokens whose place is
- * negative, behind the page list or in a page outside the cache are left out and flagged.  Two
- * tokens with the same place (a page that two sequences share): either one's row ends there. */
+ * negative, behind the page list or in a page outside the cache are left out and flagged.  Of two
+ * tokens with the same place (a page that two sequences share) either one's bytes end there. */
 moe_status moe_kv_append(moe_attn *a, const moe_kv_cache *kv, const moe_seq_batch *seqs, const void *k,
                          const void *v, int in_type, int64_t k_row_stride, int64_t v_row_stride, void *stream);
 
@@ -328,7 +331,8 @@ moe_status moe_kv_append(moe_attn *a, const moe_kv_cache *kv, const moe_seq_batc
  *   o[b][h] = sum_j softmax_j(scale * q[b][h] . K_j) V_j,   lse[b][h] = log(sum_j exp(scale * q[b][h] . K_j))
  * q, o: rows of n_q_heads heads, q_row_stride / o_row_stride elements apart (multiples of 8,
  * 16-byte aligned), head_dim contiguous.  lse f32 [n_rows][n_q_heads] or NULL.  Scores, maxima,
- * sums and products are held in f32.  A row that sees no token (kv_len 0) gets o = 0 and lse =
+ * sums and products are held in f32, and the sums are divided at the end: BF16 values whose
+ * absolute sum over the seen tokens passes 2^119 can leave its range on the way.  A row that sees no token (kv_len 0) gets o = 0 and lse =
  * -inf.  Tokens not cached (behind kv_len) are never used, whatever their places hold.  A length
  * below 0 or behind the page list is taken as the nearest in range, and the tokens of a page
  * outside the cache are left out; both are flagged (moe_attn_flags).  o may be q itself
@@ -340,7 +344,8 @@ moe_status moe_attn_decode(moe_attn *a, const moe_kv_cache *kv, const moe_seq_ba
 /* The same for packed prompts or pieces of them: row i of sequence b (n_b rows) sees the tokens
  * 0 .. kv_len[b] - n_b + i, so a prompt, and a prompt's next piece over what is cached already.
  * Rows in front of the cache (kv_len[b] < n_b) see nothing.  A token that a row does not see does
- * not reach its output, whatever it holds (infinities and NaN too). */
+ * not reach its output, whatever it holds (infinities and NaN too).  Below 2^24 workgroups:
+ * (n_rows * group / 128 + n_seqs) * n_kv_heads, group = n_q_heads / n_kv_heads. */
 moe_status moe_attn_prompt(moe_attn *a, const moe_kv_cache *kv, const moe_seq_batch *seqs, const void *q,
                            int64_t q_row_stride, float scale, void *o, int64_t o_row_stride, float *lse,
                            void *stream);

@@ -524,7 +524,12 @@ class AttnContext:
         if q.dtype != self.dtype:
             raise ValueError(f"q of {q.dtype}: the context's dtype is {self.dtype}")
         if o is None:
-            o = torch.empty_like(q, memory_format=torch.contiguous_format)
+            if stream is None:
+                o = torch.empty_like(q, memory_format=torch.contiguous_format)
+            else:  # of the memory that the call's stream may use
+                with torch.cuda.stream(stream if isinstance(stream, torch.cuda.Stream)
+                                       else torch.cuda.ExternalStream(stream, self.device)):
+                    o = torch.empty_like(q, memory_format=torch.contiguous_format)
             os_ = self.n_q_heads * self.head_dim
         else:
             os_ = self._rows("o", o, batch, self.n_q_heads)

@@ -73,6 +73,8 @@ moe_status common_args(const char *fn, moe_attn *a, const moe_kv_cache *kv, cons
         if (v < g.head_dim || (v & 7) || v > ((int64_t)1 << 40) || kv->token_stride > (1 << 24))
             return fail(MOE_EINVAL, "%s: cache stride %lld (multiples of 8, head_dim=%d at least; token_stride at most 2^24)", fn,
                         (long long)v, g.head_dim);
+    if (kv->n_pages > ((int64_t)1 << 46) / kv->page_stride)
+        return fail(MOE_EINVAL, "%s: %d pages %lld elements apart", fn, kv->n_pages, (long long)kv->page_stride);
     // steps of 32 tokens, of every sequence and head, are counted in 32 bits
     const int64_t blocks = (int64_t)g.n_kv_heads * ((g.n_q_heads / g.n_kv_heads + DEC_HEADS - 1) / DEC_HEADS);
     if ((((int64_t)s->max_pages << a->page_shift) / 32 + 1) * s->n_seqs * blocks >= ((int64_t)1 << 31))
@@ -114,18 +116,20 @@ moe_status attn_call(const char *fn, moe_attn *a, const moe_kv_cache *kv, const 
     if (q_stride < row || (q_stride & 7) || o_stride < row || (o_stride & 7))
         return fail(MOE_EINVAL, "%s: row strides %lld and %lld (multiples of 8, %lld at least)", fn,
                     (long long)q_stride, (long long)o_stride, (long long)row);
-    if (!std::isfinite(scale)) return fail(MOE_EINVAL, "%s: scale is not finite", fn);
+    c.scale_log2 = (float)(scale * 1.4426950408889634);
+    if (!std::isfinite(c.scale_log2)) return fail(MOE_EINVAL, "%s: scale %g", fn, (double)scale);
     if (s->n_seqs == 0 || s->n_rows == 0) return ok();
     if (!q || !o) return fail(MOE_EINVAL, "%s: null argument", fn);
     if (!aligned(q, 16) || !aligned(o, 16) || !aligned(lse, 4))
         return fail(MOE_EINVAL, "%s: misaligned pointer (q and o need 16 bytes)", fn);
     if (q == o && q_stride != o_stride) return fail(MOE_EINVAL, "%s: o is q with another row stride", fn);
+    if (c.row_start && prompt_places(c) >= 1 << 24) // 256 threads each: below 2^32
+        return fail(MOE_EINVAL, "%s: %d rows of %d heads in %d sequences are too many", fn, s->n_rows, c.hq, s->n_seqs);
     c.q = q;
     c.q_stride = q_stride;
     c.o = o;
     c.o_stride = o_stride;
     c.lse = lse;
-    c.scale_log2 = (float)(scale * 1.4426950408889634);
     c.part = a->part;
     c.part_ml = a->part_ml;
     c.part_rows = a->part_rows;
@@ -175,9 +179,9 @@ moe_status moe_attn_create(int device, const moe_attn_config *cfg, moe_attn **ou
     if (hipDeviceGetAttribute(&ncu, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess || ncu < 1) ncu = 1;
     a->n_cu = ncu;
     a->n_wg = 2 * ncu < DEC_MAX_WG ? 2 * ncu : DEC_MAX_WG;
-    // decode: two slots a workgroup; prompt: 3.5 pieces for each place on the card at most (prompt_d)
+    // decode: two slots a workgroup; prompt: a piece for each workgroup on the card (prompt_d)
     const int64_t dec_rows = (int64_t)a->n_wg * 2 * DEC_HEADS;
-    const int64_t prompt_rows = (int64_t)ncu * (g.head_dim == 256 ? 1 : 2) * 7 / 2 * PR_ROWS;
+    const int64_t prompt_rows = (int64_t)ncu * (g.head_dim == 256 ? 1 : 2) * PR_ROWS;
     a->part_rows = dec_rows > prompt_rows ? dec_rows : prompt_rows;
     struct Part {
         void **dst;

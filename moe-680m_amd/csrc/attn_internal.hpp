@@ -46,6 +46,10 @@ constexpr int DEC_WAVE_TOK = 32;
 constexpr int DEC_MAX_WG = 1024;
 // Prompt: (token, head) rows of a workgroup.
 constexpr int PR_ROWS = 128;
+// Workgroups of a prompt's rows however these are divided: each sequence's last tile may be short.
+inline int64_t prompt_places(const AttnArgs &a) {
+    return ((int64_t)a.n_rows * a.group / PR_ROWS + a.n_seqs) * a.hkv;
+}
 
 struct AppendArgs {
     const uint8_t *src[2];    // new keys, new values

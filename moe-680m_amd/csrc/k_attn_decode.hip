@@ -84,11 +84,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
     const int owner = __builtin_ctzll(__ballot(incl * ng > lo));
     uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), owner); // steps before b, of one unit each
     int b = owner * per, nt = uniform(seq_steps(a, b, cap));
-    while ((at + nt) * ng <= lo) {
+    while ((at + nt) * ng <= lo && b + 1 < a.n_seqs) {
         at += nt;
         nt = uniform(seq_steps(a, ++b, cap));
     }
-    int hb = (int)((lo - at * ng) / (uint32_t)nt);
+    // (a head block or sequence out of range, here and below: the lengths changed during the call)
+    int hb = min((int)((lo - at * ng) / (uint32_t)nt), ng - 1);
     uint32_t unit = at * ng + hb * nt; // first step of unit (b, hb)
 
     // a unit's first query head and heads
@@ -283,7 +284,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
         unit += nt; // the next unit
         if (++hb == ng) {
             hb = 0;
-            nt = uniform(seq_steps(a, ++b, cap));
+            if (++b >= a.n_seqs) break;
+            nt = uniform(seq_steps(a, b, cap));
         }
     }
     if (bad && lane == 0) raise(a.flags, MOE_DEVFLAG_BAD_PAGE);
@@ -303,7 +305,7 @@ __global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_
     const Piece pc = {ldc(&a.piece[blockIdx.x].b), ldc(&a.piece[blockIdx.x].hb), ldc(&a.piece[blockIdx.x].w0),
                       ldc(&a.piece[blockIdx.x].n)};
     const int n = pc.n;
-    if (n < 2) return;
+    if (n < 2 || pc.b >= a.n_seqs) return; // (an earlier call's: the lengths changed during this one)
     const int tid = threadIdx.x, lane = tid & 63;
     const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS;
     const int h0 = pc.hb / gb * a.group + pc.hb % gb * DEC_HEADS; // the unit's first query head, and its heads

@@ -88,7 +88,8 @@ struct Place {
 
 // Place number blockIdx.x; false where there is none.  Tile numbers run over the sequences, the last one
 // first (it sees the most tokens); the key-value head is the fastest index, so that a head's tiles
-// share an XCD's L2.
+// share an XCD's L2.  (No loop runs on and no index leaves its array if the lengths and rows should
+// change under the call.)
 __device__ __forceinline__ bool find_place(const AttnArgs &a, int lane, bool snake, bool flag, Place &pl) {
     const int cap = a.max_pages << a.page_shift;
     const int per = (a.n_seqs + 63) / 64;
@@ -125,7 +126,7 @@ __device__ __forceinline__ bool find_place(const AttnArgs &a, int lane, bool sna
     for (;; ++b) {
         sr = seq_rows(a, uniform(b));
         const uint32_t n = tiles(sr.n);
-        if (want < at + n) break;
+        if (want < at + n || b + 1 >= a.n_seqs) break;
         at += n;
     }
     pl.b = uniform(b);
@@ -133,7 +134,8 @@ __device__ __forceinline__ bool find_place(const AttnArgs &a, int lane, bool sna
     pl.hk = blockIdx.x - nth * a.hkv;
     pl.f0 = (int)(want - at) * PR_ROWS;
     pl.nf = uniform(sr.n) * a.group;
-    pl.first_pos = (int64_t)ldc(a.kv_len + pl.b) - ldc(a.row_start + pl.b + 1) + pl.r0;
+    if (pl.f0 >= pl.nf) return false; // (the arrays changed during the call)
+    pl.first_pos = (int64_t)min(max(ldc(a.kv_len + pl.b), 0), cap) - ldc(a.row_start + pl.b + 1) + pl.r0;
     pl.full = uniform(seen_by(a, pl.first_pos, pl.f0));
     pl.ext = uniform(seen_by(a, pl.first_pos, min(pl.f0 + PR_ROWS, pl.nf) - 1));
     pl.chunk = 1 << 30;
@@ -438,7 +440,7 @@ __global__ __launch_bounds__(256) void k_attn_prompt_join(AttnArgs a) {
     const int tid = threadIdx.x;
     Place pl;
     if (!find_place(a, tid & 63, D < 256, false, pl)) return;
-    const int tiles = (pl.ext + BN - 1) / BN, n = (tiles + pl.chunk - 1) / pl.chunk;
+    const int tiles = (pl.ext + BN - 1) / BN, n = min(a.splits, (tiles + pl.chunk - 1) / pl.chunk);
     if (n < 2) return;
     for (int i = tid; i < JOIN_ROWS * TPR; i += 256) {
         const int r = blockIdx.y * JOIN_ROWS + i / TPR, d = i % TPR * 4;
@@ -476,8 +478,7 @@ __global__ __launch_bounds__(256) void k_attn_prompt_join(AttnArgs a) {
 template <typename T, int D>
 hipError_t prompt_d(const AttnArgs &args, hipStream_t st) {
     AttnArgs a = args;
-    // tiles of the rows however they are divided: each sequence's last one may be short
-    const int64_t places = ((int64_t)a.n_rows * a.group / PR_ROWS + a.n_seqs) * a.hkv;
+    const int64_t places = prompt_places(a);
     // A quarter of the card's workgroup slots or less: the longest rows are cut into pieces, as many as
     // fill them once.  64 rows of 16 heads of 256 over 32k tokens: 1144 -> 78 us (99 us cut to fill them
     // twice), 256 rows over 16k 583 -> 109 us.  With more places the partial rows cost what the pieces

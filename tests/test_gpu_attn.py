@@ -596,3 +596,286 @@ def test_refusals(gpu):
     ctx.close()
     with pytest.raises(ValueError):
         ctx.attn_decode(cache, batch, q)
+
+
+@pytest.mark.parametrize("heads", [(200, 1, 64), (256, 1, 128), (36, 2, 256), (256, 256, 64)])
+def test_decode_many_heads(gpu, heads):
+    """Head blocks of 16, the last one short, and as many key-value heads as there may be."""
+    log(f"decode heads {heads}")
+    run_decode(gpu, Setup(*heads, 16, "f16", [200, 0, 33], seed=30))
+
+
+def test_prompt_and_append_of_many_sequences(gpu):
+    """More sequences than lanes, many without rows: rows, places and pages are found."""
+    import torch
+    log("prompt of 700 sequences")
+    rows = [(7 * b) % 4 for b in range(700)]
+    before = [(5 * b) % 23 for b in range(700)]
+    s = Setup(2, 1, 64, 16, "bf16", [r + c for r, c in zip(rows, before)], rows, seed=31, extra_rows=2)
+    run_decode(gpu, s)
+    k, v = s.pools(filled=False)
+    new_k = torch.cat([K[c:] for K, c in zip(s.K, before)] + [torch.full((2, 1, 64), 5.0, dtype=s.type)])
+    new_v = torch.cat([V[c:] for V, c in zip(s.V, before)] + [torch.full((2, 1, 64), 5.0, dtype=s.type)])
+    ctx = s.context(gpu)
+    ctx.kv_append(gpu.KVCache(k, v), s.seqs(gpu), new_k.cuda(), new_v.cuda())
+    k, v = k.cpu(), v.cpu()
+    places = 0
+    for b, (r, c) in enumerate(zip(rows, before)):
+        for t in range(c, c + r):
+            pg = int(s.pages[b, t // 16])
+            assert torch.equal(k[pg, :, t % 16], s.K[b][t]) and torch.equal(v[pg, :, t % 16], s.V[b][t])
+            places += 1
+    assert int((~torch.isnan(k)).sum()) == int((~torch.isnan(v)).sum()) == places * 64
+    assert ctx.device_flags() == 0
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+def test_scores_that_keep_growing(gpu, type):
+    """Each key's score is above the one before by 0.5: the running maximum is raised again and again."""
+    import torch
+    log(f"growing scores {type}")
+    for rows in (None, [300]):
+        s = Setup(4, 2, 64, 16, type, [300], rows, seed=32)
+        s.q[:] = 1.0
+        s.K[0][:] = (torch.arange(300).view(-1, 1, 1) * (0.5 * 8 / 64)).to(s.type)
+        run_decode(gpu, s)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("-inf")])
+def test_unseen_values_over_a_long_cache(gpu, bad):
+    """Few rows over a cache that is cut into pieces: the last token's value reaches the last row only."""
+    import torch
+    log(f"{bad} at the end of a long cache")
+    s = Setup(4, 2, 128, 16, "f16", [9003], [3], seed=33)
+    want, bound, _, _ = s.reference()
+    s.V[0][9002, :, 7] = bad
+    o, _, flags = run_decode(gpu, s, ref=False)
+    check("o", o[:2], want[:2], bound[:2])
+    assert flags == 0
+    assert torch.isnan(o[2, :, 7]).all() if math.isnan(bad) else (o[2, :, 7] == bad).all()
+    o[2, :, 7] = 0
+    want[2, :, 7] = 0
+    check("o", o, want, bound)
+
+
+def test_bad_page_beside_an_infinite_value(gpu):
+    """A tile that all rows see whole, with a page outside the cache and an infinity in another page."""
+    log("bad page and an infinity")
+    s = Setup(4, 2, 64, 16, "f16", [200], [10], seed=34)
+    s.V[0][5, :, 3] = float("inf")
+    k, v = s.pools()
+    ctx = s.context(gpu)
+    batch = s.seqs(gpu)
+    batch.pages[0, 2] = -7  # tokens 32..47 of the first tile
+    o = ctx.attn_prompt(gpu.KVCache(k, v), batch, s.q.cuda())
+    assert ctx.device_flags() == gpu.DEVFLAG_BAD_PAGE
+    assert (o[:, :, 3] == math.inf).all()
+    keep = list(range(32)) + list(range(48, 200))
+    ref = Setup(4, 2, 64, 16, "f16", [184], [10], seed=34)
+    ref.q, ref.K, ref.V = s.q, [s.K[0][keep]], [s.V[0][keep].clone()]
+    ref.V[0][5, :, 3] = 0.0
+    want, bound, _, _ = ref.reference()
+    o[:, :, 3] = 0
+    want[:, :, 3] = 0
+    check("o", o, want, bound)
+
+
+@pytest.mark.parametrize("rows", [None, [5, 60]])
+def test_on_another_stream(gpu, rows):
+    """stream= names another stream than the current one, as an object or a handle; the current stream
+    is busy meanwhile."""
+    import torch
+    log(f"another stream, rows {rows}")
+    s = Setup(*MODEL, 16, "bf16", [5000, 300], rows, seed=35)
+    k, v = s.pools()
+    ctx = s.context(gpu)
+    call = ctx.attn_decode if rows is None else ctx.attn_prompt
+    cache, batch, q = gpu.KVCache(k, v), s.seqs(gpu), s.q.cuda()
+    good = call(cache, batch, q)
+    torch.cuda.synchronize()
+    other = torch.cuda.Stream()
+    busy = torch.randn(2048, 2048, device="cuda")
+    for _ in range(5):
+        for st in (other, other.cuda_stream):
+            busy = busy @ busy * 1e-3
+            o = call(cache, batch, q, stream=st)
+            other.synchronize()
+            assert torch.equal(o, good)
+    torch.cuda.synchronize()
+
+
+def test_scales_and_pools_out_of_range(gpu):
+    import ctypes
+    import torch
+    log("scale and pool limits")
+    ctx = gpu.AttnContext(4, 2, 64, 16, 4)
+    k = torch.zeros((3, 2, 16, 64), dtype=torch.float16, device="cuda")
+    batch = gpu.SeqBatch(torch.zeros((1, 1), dtype=torch.int32, device="cuda"),
+                         torch.ones(1, dtype=torch.int32, device="cuda"))
+    q = torch.zeros((1, 4, 64), dtype=torch.float16, device="cuda")
+    cache = gpu.KVCache(k, k.clone())
+    for scale in (3e38, -3e38, float("-inf")):
+        with pytest.raises(gpu.MoeError):
+            ctx.attn_decode(cache, batch, q, scale=scale)
+    ctx.attn_decode(cache, batch, q, scale=1e37)
+    cache._c.page_stride = 1 << 40
+    cache._c.n_pages = 1 << 20
+    with pytest.raises(gpu.MoeError):
+        ctx.attn_decode(cache, batch, q)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("cut", [False, True])
+def test_prompt_lengths_out_of_range(gpu, cut):
+    """A length behind the page list is the list's end, also for the places of the rows; one below 0 is 0."""
+    import torch
+    log(f"prompt lengths out of range, {'a long cache' if cut else 'short'}")
+    s = Setup(4, 2, 64, 16, "bf16", [9008 if cut else 96, 50], [33, 20], seed=36, pad_pages=0)
+    k, v = s.pools()
+    ctx = s.context(gpu)
+    cache, batch, q = gpu.KVCache(k, v), s.seqs(gpu), s.q.cuda()
+    good = ctx.attn_prompt(cache, batch, q)
+    for n in (s.kv[0] + 1, s.kv[0] + 40, 2 ** 31 - 1):
+        batch.kv_len[0] = n
+        o = ctx.attn_prompt(cache, batch, q)
+        assert ctx.device_flags() == gpu.DEVFLAG_BAD_SEQ
+        assert torch.equal(o, good)
+    batch.kv_len[0] = -2 ** 31
+    o = ctx.attn_prompt(cache, batch, q)
+    assert ctx.device_flags() == gpu.DEVFLAG_BAD_SEQ
+    assert (o[:33] == 0).all()
+    check("o", o[33:], *[x[33:] for x in s.reference()[:2]])
+
+
+@pytest.mark.parametrize("heads", [(4, 2, 64), (4, 1, 128), (6, 2, 256)])
+def test_decode_pieces_of_many_units(gpu, heads):
+    """More units than workgroups, one sequence far longer than the rest: cut among many of them, and the
+    ones in the middle cut in few."""
+    log(f"decode pieces {heads}")
+    kv = [1 + (11 * b) % 40 for b in range(600)]
+    kv[311] = 30000
+    kv[100] = 2500
+    run_decode(gpu, Setup(*heads, 64, "f16", kv, seed=37))
+
+
+def test_decode_pieces_of_some_units(gpu):
+    """Fewer units than workgroups, with 512 to 2048 rows to join."""
+    log("decode pieces of 64 units")
+    run_decode(gpu, Setup(16, 1, 64, 32, "bf16", [700 + 3 * b for b in range(64)], seed=38))
+
+
+@pytest.mark.parametrize("rows", [None, [4, 1, 2]])
+def test_nothing_cached(gpu, rows):
+    log(f"lengths of zero, rows {rows}")
+    o, _, _ = run_decode(gpu, Setup(8, 2, 128, 16, "f16", [0, 0, 0], rows, seed=39))
+    assert (o == 0).all()
+
+
+@pytest.mark.parametrize("rows", [None, [7, 60], [1, 2]])
+def test_a_query_that_is_not_finite(gpu, rows):
+    """NaN and infinities in one row's query reach no other row."""
+    import torch
+    log(f"NaN queries, rows {rows}")
+    s = Setup(8, 2, 64, 16, "f16", [5000, 80], rows, seed=40)
+    want, bound, _, _ = s.reference()
+    keep = [(r, h) for r in range(s.n_rows) for h in range(8) if (r, h) not in ((0, 3), (1, 0))]
+    s.q[0, 3] = float("nan")
+    s.q[1, 0, 5] = float("inf")
+    o, _, _ = run_decode(gpu, s, ref=False)
+    r, h = torch.tensor(keep).T
+    check("o", o[r.cuda(), h.cuda()], want[r, h], bound[r, h])
+    assert torch.isnan(o[0, 3]).all()
+
+
+@pytest.mark.parametrize("rows", [None, [21, 30, 18]])
+def test_shared_pages(gpu, rows):
+    """Sequences that begin with the same pages, and one page twice in a list."""
+    import torch
+    log(f"shared pages, rows {rows}")
+    s = Setup(8, 2, 64, 16, "bf16", [100, 90, 60], rows, seed=41)
+    for b in (1, 2):  # the first 48 tokens
+        s.pages[b, :3] = s.pages[0, :3]
+        s.K[b][:48], s.V[b][:48] = s.K[0][:48], s.V[0][:48]
+    s.pages[0, 4] = s.pages[0, 3]
+    s.K[0][64:80], s.V[0][64:80] = s.K[0][48:64], s.V[0][48:64]
+    run_decode(gpu, s)
+
+
+def test_calls_in_a_row_share_the_workspace(gpu):
+    """One context, no wait between calls of different shapes: each result is that of a call alone."""
+    import torch
+    log("calls in a row")
+    sets = [Setup(4, 2, 128, 16, "f16", kv, rows, seed=42 + i) for i, (kv, rows) in enumerate([
+        ([9000], None), ([9000], [5]), ([40] * 300, None), ([8000, 3], [2, 1]), ([2000, 60, 0, 7000], None)])]
+    ctx = sets[0].context(gpu, max_seqs=300)
+    calls = []
+    for s in sets:
+        call = ctx.attn_decode if s.rows is None else ctx.attn_prompt
+        args = (gpu.KVCache(*s.pools()), s.seqs(gpu), s.q.cuda())
+        calls.append((call, args, call(*args)))
+        torch.cuda.synchronize()
+    got = [(call(*args), good) for _ in range(4) for call, args, good in calls]
+    for o, good in got:
+        assert torch.equal(o, good)
+
+
+def test_padded_batch_in_a_graph(gpu):
+    """A captured step of a fixed number of sequences, some of them not in use (length 0, no page)."""
+    import torch
+    log("padded batch")
+    full = Setup(*MODEL, 16, "f16", [700, 80, 33, 1, 500, 16], seed=43, junk=0.0)
+    k, v = full.pools()
+    cache, batch, q = gpu.KVCache(k, v), full.seqs(gpu), full.q.cuda()
+    ctx, other = full.context(gpu), full.context(gpu)
+    nk, nv = (torch.randn((6, 2, 256), device="cuda") for _ in range(2))
+    o = torch.empty_like(q)
+    g = torch.cuda.CUDAGraph()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st), torch.cuda.graph(g, stream=st):
+        ctx.attn_decode(cache, batch, q, o=o)
+    for used in (6, 3, 0, 5):
+        kv = torch.tensor(full.kv, dtype=torch.int32)
+        kv[used:] = 0
+        batch.kv_len.copy_(kv)
+        o.fill_(float("nan"))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        some = gpu.SeqBatch(batch.pages[:used], batch.kv_len[:used])
+        assert (o[used:] == 0).all()
+        if used:
+            want, bound, _, _ = full.reference()
+            check("o", o[:used], want[:used], bound[:used])
+            check("alone", other.attn_decode(cache, some, q[:used]), want[:used], bound[:used])
+        assert ctx.device_flags() == 0
+    # the write leaves an unused sequence's row out and says so
+    before = k.clone()
+    batch.kv_len.zero_()
+    ctx.kv_append(cache, batch, nk, nv)
+    assert torch.equal(k, before) and ctx.device_flags() == gpu.DEVFLAG_BAD_SEQ
+
+
+def test_most_sequences(gpu):
+    """65535 sequences of a token or none; as prompts of as many rows and heads as cannot be launched."""
+    import torch
+    log("65535 sequences")
+    n = 65535
+    ctx = gpu.AttnContext(2, 1, 64, 16, n)
+    v = torch.randn((50, 1, 16, 64), device="cuda").half()
+    k = torch.randn_like(v)
+    pages = (torch.arange(n, device="cuda", dtype=torch.int32) % 50).view(n, 1)
+    kv_len = (torch.arange(n, device="cuda", dtype=torch.int32) % 3 > 0).int()
+    q = torch.randn((n, 2, 64), device="cuda").half()
+    want = (v[pages[:, 0].long(), :, 0] * kv_len.view(n, 1, 1)).expand(n, 2, 64)
+    start = torch.arange(n + 1, device="cuda", dtype=torch.int32)
+    cache = gpu.KVCache(k, v)
+    assert torch.equal(ctx.attn_decode(cache, gpu.SeqBatch(pages, kv_len), q), want)
+    assert torch.equal(ctx.attn_prompt(cache, gpu.SeqBatch(pages, kv_len, start, n), q), want)
+    assert ctx.device_flags() == 0
+    ctx = gpu.AttnContext(256, 256, 64, 16, n)
+    k = torch.zeros((50, 256, 16, 64), dtype=torch.float16, device="cuda")
+    q = torch.zeros((n, 256, 64), dtype=torch.float16, device="cuda")
+    with pytest.raises(gpu.MoeError):
+        ctx.attn_prompt(gpu.KVCache(k, k.clone()), gpu.SeqBatch(pages, kv_len, start, n), q)
+    torch.cuda.synchronize()
