@@ -35,7 +35,8 @@ struct AttnArgs {
     Piece *piece;             // ... and the units to join
     int n_wg;                 // workgroups of a decode launch
     int n_cu;
-    int splits;               // prompt: pieces of the longest rows
+    int splits;               // prompt: most pieces of a row (1: not cut)
+    unsigned splits_below;    // ... and the most tiles of rows that are cut
     int64_t part_rows;        // rows that part and part_ml hold
 };
 

@@ -29,17 +29,24 @@ namespace {
 constexpr int BN = 64;           // tokens of a tile
 constexpr float LAZY = 8.f;      // log2 of what a weight may exceed 1 by
 constexpr int PR_MIN_CHUNK = 4;  // tiles of a piece at least
-constexpr int PR_MAX_SPLITS = 64;
+constexpr int PR_CUT_FROM = 9;   // tiles of the longest rows from which on they are cut
+constexpr int PR_MAX_SPLITS = 128;
 
+// A sequence's packed rows, inside the arrays whatever row_start holds, and its length.
 struct Rows {
-    int r0, n;
+    int r0, n, end, len; // end: row_start's own
     bool bad;
 };
-// The packed rows of sequence b, inside the arrays whatever row_start holds.
 __device__ __forceinline__ Rows seq_rows(const AttnArgs &a, int b) {
-    const int s = a.row_start[b], e = a.row_start[b + 1];
+    const int s = ldg<int>(a.row_start + b), e = ldg<int>(a.row_start + b + 1), len = ldg<int>(a.kv_len + b);
     const int r0 = min(max(s, 0), a.n_rows), r1 = min(max(e, r0), a.n_rows);
-    return {r0, r1 - r0, r0 != s || r1 != e};
+    return {r0, r1 - r0, e, len, r0 != s || r1 != e};
+}
+
+// Workgroups that are on the card at once.
+template <int D>
+__host__ __device__ __forceinline__ uint32_t slots_of(const AttnArgs &a) {
+    return a.n_cu * (D == 256 ? 1u : 2u);
 }
 
 // Tokens that the f-th (token, head) pair's row of a sequence sees, its first row's position given.
@@ -78,77 +85,96 @@ __device__ __forceinline__ void products(Read read, Product product) {
 }
 
 // A workgroup's place: PR_ROWS (token, head) pairs of sequence b, from its f0-th of nf on, of which the
-// last one sees ext tokens and the first one `full`; pieces of them, `chunk` tiles each.
+// last one sees ext tokens and the first one `full`; piece `piece` of n at most, `chunk` tiles each.
 struct Place {
     int b, r0, hk;
     int f0, nf;
     int64_t first_pos; // of the sequence's first row
     int ext, full, chunk;
+    int nth, piece, n; // nth: place number
 };
 
-// Place number blockIdx.x; false where there is none.  Tile numbers run over the sequences, the last one
-// first (it sees the most tokens); the key-value head is the fastest index, so that a head's tiles
-// share an XCD's L2.  (No loop runs on and no index leaves its array if the lengths and rows should
-// change under the call.)
-__device__ __forceinline__ bool find_place(const AttnArgs &a, int lane, bool snake, bool flag, Place &pl) {
+// This workgroup's place, or (join) place number blockIdx.x; false where there is none.  Tile numbers run
+// over the sequences, the last one first (it sees the most tokens).  Whole rows: the key-value head is the
+// fastest index, so that a head's tiles share an XCD's L2.  Rows in pieces: the tiles that read the same
+// tokens lie on one XCD (workgroups go round the XCDs in turn), side by side.  (No loop runs on and no
+// index leaves its array if the lengths and rows should change under the call.)
+template <int D, bool JOIN>
+__device__ __forceinline__ bool find_place(const AttnArgs &a, int lane, bool flag, Place &pl) {
     const int cap = a.max_pages << a.page_shift;
     const int per = (a.n_seqs + 63) / 64;
     auto tiles = [&](int n) { return ((uint32_t)n * a.group + PR_ROWS - 1) / PR_ROWS; };
     uint32_t mine = 0;
     int most = 0; // tokens that a row sees
     bool bad = false;
+    Rows sr = {};
     for (int i = 0; i < per; ++i) {
         const int b = lane * per + i;
         if (b < a.n_seqs) {
-            const Rows w = seq_rows(a, b);
-            bad |= w.bad;
-            mine += tiles(w.n);
-            if (w.n > 0) {
-                const int len = a.kv_len[b];
-                bad |= len < 0 || len > cap;
-                most = max(most, min(len, cap));
+            sr = seq_rows(a, b);
+            bad |= sr.bad;
+            mine += tiles(sr.n);
+            if (sr.n > 0) {
+                bad |= sr.len < 0 || sr.len > cap;
+                most = max(most, min(sr.len, cap));
             }
         }
     }
     if (flag && bad) raise(a.flags, MOE_DEVFLAG_BAD_SEQ);
     const uint32_t incl = wave_scan(mine);
     const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
-    const uint32_t nth = blockIdx.x / a.hkv;
+    if (total == 0) return false;
+    uint32_t nth = blockIdx.x / a.hkv; // tile number, from the end
+    pl.hk = blockIdx.x - nth * a.hkv;
+    pl.piece = 0;
+    pl.n = 1;
+    pl.chunk = 1 << 30;
+    if (a.splits > 1 && total <= a.splits_below && __any(most > (PR_CUT_FROM - 1) * BN)) {
+        for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
+        const int n = min(a.splits, (int)(slots_of<D>(a) / (total * a.hkv))), tiles = (uniform(most) + BN - 1) / BN;
+        pl.chunk = max(PR_MIN_CHUNK, (tiles + n - 1) / n);
+        pl.n = max(1, (tiles + pl.chunk - 1) / pl.chunk);
+        if (!JOIN) {
+            const uint32_t jobs = total * a.hkv * pl.n, per_xcd = (jobs + 7) / 8;
+            const uint32_t y = blockIdx.x / 8, job = blockIdx.x % 8 * per_xcd + y;
+            if (y >= per_xcd || job >= jobs) return false;
+            const uint32_t s = job / total;
+            nth = job - s * total;
+            pl.piece = s / a.hkv;
+            pl.hk = s - pl.piece * a.hkv;
+        }
+    }
     if (nth >= total) return false;
+    pl.nth = nth * a.hkv + pl.hk;
     uint32_t want = total - 1 - nth;
     // All at work at once, two on some CUs: there the lighter one is to lie beside the heavier one.
     const uint32_t first = a.n_cu / a.hkv; // (head groups of) tiles that take a CU each
-    if (snake && total > first && total * a.hkv <= 2u * a.n_cu && nth >= first) want = nth - first;
+    if (D < 256 && pl.n == 1 && total > first && total * a.hkv <= 2u * a.n_cu && nth >= first) want = nth - first;
     const int owner = __builtin_ctzll(__ballot(incl > want));
     uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), owner);
-    int b = owner * per;
-    Rows sr;
-    for (;; ++b) {
-        sr = seq_rows(a, uniform(b));
-        const uint32_t n = tiles(sr.n);
-        if (want < at + n || b + 1 >= a.n_seqs) break;
-        at += n;
-    }
-    pl.b = uniform(b);
-    pl.r0 = uniform(sr.r0);
-    pl.hk = blockIdx.x - nth * a.hkv;
+    int b = owner * per, from = owner; // (one sequence a lane: the owner has it)
+    if (per > 1)
+        for (from = 0;; ++b) {
+            sr = seq_rows(a, b);
+            const uint32_t n = uniform(tiles(sr.n));
+            if (want < at + n || b + 1 >= a.n_seqs) break;
+            at += n;
+        }
+    auto of = [&](int v) { return __builtin_amdgcn_readlane(v, from); };
+    pl.b = b;
+    pl.r0 = of(sr.r0);
     pl.f0 = (int)(want - at) * PR_ROWS;
-    pl.nf = uniform(sr.n) * a.group;
+    pl.nf = of(sr.n) * a.group;
     if (pl.f0 >= pl.nf) return false; // (the arrays changed during the call)
-    pl.first_pos = (int64_t)min(max(ldc(a.kv_len + pl.b), 0), cap) - ldc(a.row_start + pl.b + 1) + pl.r0;
+    pl.first_pos = (int64_t)min(max(of(sr.len), 0), cap) - of(sr.end) + pl.r0;
     pl.full = uniform(seen_by(a, pl.first_pos, pl.f0));
     pl.ext = uniform(seen_by(a, pl.first_pos, min(pl.f0 + PR_ROWS, pl.nf) - 1));
-    pl.chunk = 1 << 30;
-    if (a.splits > 1) {
-        for (int o = 1; o < 64; o <<= 1) most = max(most, __shfl_xor(most, o));
-        pl.chunk = uniform(max(PR_MIN_CHUNK, ((most + BN - 1) / BN + a.splits - 1) / a.splits));
-    }
     return true;
 }
 
-// Partial rows of piece `piece` of place blockIdx.x.
-__device__ __forceinline__ size_t part_row(const AttnArgs &a, int piece) {
-    return ((size_t)blockIdx.x * a.splits + piece) * PR_ROWS;
+// A place's partial rows of piece `piece`.
+__device__ __forceinline__ size_t part_row(const Place &pl, int piece) {
+    return ((size_t)pl.nth * pl.n + piece) * PR_ROWS;
 }
 
 // f16: 2^(SHIFT + LAZY) is in range.
@@ -174,10 +200,10 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
     Place pl;
-    if (!find_place(a, lane, D < 256, blockIdx.x == 0 && blockIdx.y == 0 && wave == 0, pl)) return;
+    if (!find_place<D, false>(a, lane, blockIdx.x == 0 && wave == 0, pl)) return;
     // this piece's tiles [t, nt); the first one also where no token is seen, to write the rows
-    const int tiles = (pl.ext + BN - 1) / BN, first_t = (int)min((int64_t)blockIdx.y * pl.chunk, (int64_t)1 << 30);
-    if (blockIdx.y > 0 && first_t >= tiles) return;
+    const int tiles = (pl.ext + BN - 1) / BN, first_t = pl.piece * pl.chunk;
+    if (pl.piece > 0 && first_t >= tiles) return;
     const int nt = min(tiles, first_t + pl.chunk), ext = pl.ext;
     const bool whole = tiles <= pl.chunk;
     if (tid == 0) s_bad = 0;
@@ -388,7 +414,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
     const float sum = l + __shfl_xor(l, 32);
     if (!whole) {
         if (!valid) return;
-        const size_t pr = part_row(a, blockIdx.y) + wave * 32 + r;
+        const size_t pr = part_row(pl, pl.piece) + wave * 32 + r;
         if (h == 0) *(f32x2 *)(a.part_ml + 2 * pr) = f32x2{m, sum};
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
@@ -431,31 +457,36 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
     }
 }
 
-// The partial rows of places that were cut into pieces, JOIN_ROWS a workgroup: sum_p f_p x_p / sum_p f_p l_p,
-// f_p = 2^(m_p - max m), in the pieces' order.
+// The partial rows of places that were cut into pieces: sum_p f_p x_p / sum_p f_p l_p, f_p = 2^(m_p - max m),
+// the same order every time.  One row a workgroup (gridDim.y = PR_ROWS): a thread takes four elements of
+// every PG-th piece, and the threads' sums are joined through LDS.  More rows: a thread takes four
+// elements of a row through all pieces.
 constexpr int JOIN_ROWS = 8, JOIN_B = 8;
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_attn_prompt_join(AttnArgs a) {
-    constexpr int TPR = D / 4;
-    const int tid = threadIdx.x;
+    constexpr int TPR = D / 4, PG = 256 / TPR;
+    __shared__ f32x4 s_x[PG][TPR];
+    __shared__ f32x2 s_ml[PG];
+    const int tid = threadIdx.x, i = tid % TPR, g = tid / TPR;
     Place pl;
-    if (!find_place(a, tid & 63, D < 256, false, pl)) return;
-    const int tiles = (pl.ext + BN - 1) / BN, n = min(a.splits, (tiles + pl.chunk - 1) / pl.chunk);
+    if (!find_place<D, true>(a, tid & 63, false, pl)) return;
+    const int tiles = (pl.ext + BN - 1) / BN, n = min(pl.n, (tiles + pl.chunk - 1) / pl.chunk);
     if (n < 2) return;
-    for (int i = tid; i < JOIN_ROWS * TPR; i += 256) {
-        const int r = blockIdx.y * JOIN_ROWS + i / TPR, d = i % TPR * 4;
-        const int pair = pl.f0 + r;
-        if (pair >= pl.nf) continue;
-        const int tok = pair / a.group, head = pl.hk * a.group + pair - tok * a.group;
+    const bool one = gridDim.y == PR_ROWS;
+    const int rows = PR_ROWS / gridDim.y, step = one ? PG : 1;
+    for (int x0 = one ? 0 : g; x0 < rows; x0 += PG) {
+        const int r = blockIdx.y * rows + x0, pair = pl.f0 + r;
+        if (pair >= pl.nf) return; // (one: all threads)
         float M = -INFINITY, L = 0.f;
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
-        for (int p = 0; p < n; p += JOIN_B) {
+        for (int p = one ? g : 0; p < n; p += JOIN_B * step) {
             f32x2 ml[JOIN_B];
             f32x4 v[JOIN_B];
 #pragma unroll
             for (int j = 0; j < JOIN_B; ++j) {
-                ml[j] = p + j < n ? ldg<f32x2>(a.part_ml + 2 * (part_row(a, p + j) + r)) : f32x2{-INFINITY, 0.f};
-                v[j] = p + j < n ? ldg<f32x4>(a.part + (part_row(a, p + j) + r) * D + d) : f32x4{};
+                const int q = p + j * step;
+                ml[j] = q < n ? ldg<f32x2>(a.part_ml + 2 * (part_row(pl, q) + r)) : f32x2{-INFINITY, 0.f};
+                v[j] = q < n ? ldg<f32x4>(a.part + (part_row(pl, q) + r) * D + 4 * i) : f32x4{};
             }
             float mn = M;
 #pragma unroll
@@ -466,34 +497,54 @@ __global__ __launch_bounds__(256) void k_attn_prompt_join(AttnArgs a) {
             x *= f;
 #pragma unroll
             for (int j = 0; j < JOIN_B; ++j) {
-                const float g = exp2_(ml[j].x - base_of(M));
-                L += g * ml[j].y;
-                x += g * v[j];
+                const float w = exp2_(ml[j].x - base_of(M));
+                L += w * ml[j].y;
+                x += w * v[j];
             }
         }
-        put_row<T>(a, pl.r0 + tok, head, D, d, x, M, L, SHIFT<T>);
+        if (one) {
+            s_x[g][i] = x;
+            if (i == 0) s_ml[g] = f32x2{M, L};
+            __syncthreads();
+            if (g) return;
+            const float m0 = M;
+            for (int k = 1; k < PG; ++k) M = fmaxf(M, s_ml[k].x);
+            const float f = exp2_(m0 - base_of(M));
+            L *= f;
+            x *= f;
+            for (int k = 1; k < PG; ++k) {
+                const float w = exp2_(s_ml[k].x - base_of(M));
+                L += w * s_ml[k].y;
+                x += w * s_x[k][i];
+            }
+        }
+        const int tok = pair / a.group, head = pl.hk * a.group + pair - tok * a.group;
+        put_row<T>(a, pl.r0 + tok, head, D, 4 * i, x, M, L, SHIFT<T>);
     }
 }
 
 template <typename T, int D>
 hipError_t prompt_d(const AttnArgs &args, hipStream_t st) {
     AttnArgs a = args;
-    const int64_t places = prompt_places(a);
-    // A quarter of the card's workgroup slots or less: the longest rows are cut into pieces, as many as
-    // fill them once.  64 rows of 16 heads of 256 over 32k tokens: 1144 -> 78 us (99 us cut to fill them
-    // twice), 256 rows over 16k 583 -> 109 us.  With more places the partial rows cost what the pieces
-    // gain: a prompt of 1024 rows of 32/8 heads of 128 (half the slots) 32 us whole, 44 us cut in two.
-    const int64_t slots = (int64_t)a.n_cu * (D == 256 ? 1 : 2), cap = (int64_t)a.max_pages << a.page_shift;
+    const int64_t places = prompt_places(a), slots = slots_of<D>(a), cap = (int64_t)a.max_pages << a.page_shift;
+    // A quarter of the card's workgroup slots or less, and PR_CUT_FROM tiles: the rows are cut into pieces, as
+    // many as fill the slots once.  64 rows of 16/2 heads of 256 over 32k tokens: 1144 -> 62 us (99 us cut to
+    // fill them twice, by an earlier join).  With more places the partial rows cost what the pieces gain:
+    // 1024 rows of 32/8 heads of 128 (half the slots) 32 us whole, 44 us cut in two.  Of 9 tiles (64 rows
+    // after 512) 28.0 -> 24.4 us and, 32/8 heads of 128, 18.3 -> 16.7 us; of 8 (512 rows) 26.6 -> 27.9 and 17.4 ->
+    // 23.2 us.  (The worst that the rule does: 512 rows after 256 of 32/8 heads of 128, 22.8 -> 27.9 us; after
+    // 2048, 61 -> 42 us.)  The kernels count the tiles themselves, so sequences without rows do not matter;
+    // whether it can be is known here, and the second launch left out otherwise.
+    a.splits_below = (unsigned)(slots / 4 / a.hkv);
     const int64_t useful = (cap + BN * PR_MIN_CHUNK - 1) / (BN * PR_MIN_CHUNK);
     a.splits = 1;
-    if (4 * places <= slots) {
-        int64_t n = slots / places;
-        if (n > useful) n = useful;
-        if (n > PR_MAX_SPLITS) n = PR_MAX_SPLITS;
-        if (n * places * PR_ROWS <= a.part_rows) a.splits = (int)n;
+    if (cap > (PR_CUT_FROM - 1) * BN && (int64_t)a.n_rows * a.group <= (int64_t)a.splits_below * PR_ROWS)
+        a.splits = (int)(useful < PR_MAX_SPLITS ? useful : PR_MAX_SPLITS);
+    k_attn_prompt<T, D><<<(unsigned)(a.splits > 1 && places < slots + 7 ? slots + 7 : places), 256, 0, st>>>(a);
+    if (a.splits > 1) {
+        const int64_t cut = (int64_t)a.splits_below * a.hkv, x = places < cut ? places : cut;
+        k_attn_prompt_join<T, D><<<dim3((unsigned)x, PR_ROWS / (x > 16 ? JOIN_ROWS : 1)), 256, 0, st>>>(a);
     }
-    k_attn_prompt<T, D><<<dim3((unsigned)places, a.splits), 256, 0, st>>>(a);
-    if (a.splits > 1) k_attn_prompt_join<T, D><<<dim3((unsigned)places, PR_ROWS / JOIN_ROWS), 256, 0, st>>>(a);
     return hipGetLastError();
 }
 

@@ -879,3 +879,21 @@ def test_most_sequences(gpu):
     with pytest.raises(gpu.MoeError):
         ctx.attn_prompt(gpu.KVCache(k, k.clone()), gpu.SeqBatch(pages, kv_len, start, n), q)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("heads", [(6, 3, 64), (10, 5, 128), (4, 1, 256)])
+def test_cut_prompts_of_odd_heads_in_a_padded_batch(gpu, heads):
+    """Few rows over long caches, among many sequences without rows; pieces that do not divide by 8."""
+    import torch
+    log(f"cut prompts {heads}")
+    kv, rows = [0] * 40, [0] * 40
+    for b, n, r in ((3, 7001, 37), (17, 30, 30), (18, 2600, 5), (39, 577, 1)):
+        kv[b], rows[b] = n, r
+    kv[20] = 4000  # cached tokens, no new row
+    run_decode(gpu, Setup(*heads, 32, "f16", kv, rows, seed=50, extra_rows=4))
+
+
+@pytest.mark.parametrize("n", [511, 512, 513, 576, 577])
+def test_prompt_around_the_length_that_is_cut(gpu, n):
+    log(f"prompt of 3 rows, {n} cached")
+    run_decode(gpu, Setup(8, 2, 64, 16, "bf16", [n, 100], [3, 60], seed=51))
