@@ -104,8 +104,14 @@ __device__ __forceinline__ void lds_loaded() { asm volatile("s_waitcnt vmcnt(0)"
 // The transposing LDS read: among 16 lanes, lane 4 j + c addresses elements 4c..4c+3 of row j, lane i gets
 // element i of rows 0..3.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ u32x2 lds_read_tr(const uint8_t *p) {
+__device__ __forceinline__ u32x2 lds_read_tr(const MOE_LDS uint8_t *p) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((MOE_LDS s16x4 *)p));
+}
+// An LDS address held in a register: reads add their constants (16 bits) to it in the instruction.
+__device__ __forceinline__ const MOE_LDS uint8_t *lds_at(const void *base, uint32_t off) {
+    const MOE_LDS uint8_t *p = (const MOE_LDS uint8_t *)base + off;
+    asm("" : "+v"(p));
+    return p;
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }

@@ -12,14 +12,21 @@
 //       O^T[d][row] += V^T P^T       S^T's register layout is P^T's operand layout with the tokens of 16
 //                                    in the order {0-3, 8-11}, {4-7, 12-15}; V^T is stored in that order
 //   * K and V tiles of BN tokens go straight to LDS (no registers), two buffers, one barrier a tile; the
-//     next tile's loads are under way while this one is worked on.  V^T is read by the transposing LDS
+//     next tile's loads go out between this one's score products.  V^T is read by the transposing LDS
 //     load: of 16 lanes, lane 4 j + c gives the address of elements 4c..4c+3 of token j, lane d gets
-//     element d of tokens 0..3.  A row's 16-byte chunks are stored at chunk ^ f(token), f = token & 7 for K
-//     and 2 (token & 3) for V, so that all reads are free of bank conflicts.
+//     element d of tokens 0..3.  A row's 16-byte chunks are stored at chunk ^ f(token), f = token & 15 for K
+//     (& 7 at D = 64) and 2 (token & 3) for V, so that all reads are free of bank conflicts.
+//   * Of the weights only those of the first 16 tokens are computed before the output's products, the others
+//     between these.
 //   * The running maximum is only raised when a row's new one exceeds it by more than 2^8: until then
 //     the weights stay below 2^(8 + SHIFT) and no output is rescaled.
 //   * Too few rows to fill the card (a piece of a prompt over a long cache, short prompts): the tokens of
 //     the longest rows are cut into pieces, whose partial rows a second launch joins.
+// At D = 256 a wave has a SIMD for itself (128 registers of outputs, 64 of queries), so what it does between
+// the products adds to their time: a prompt of 4096 rows of 16/2 heads 142 us, 969 TFLOP/s, where a matrix
+// product of 8192^3 reaches 1221.  At D <= 128 two workgroups share a CU: 8192 rows of 32/8 heads of 128 529 us,
+// 1039 TFLOP/s.  (All loads before the products, all weights before theirs, the maximum's swap through
+// LDS: 167 and 553 us.)
 #include "attn_device.hpp"
 
 namespace moe {
@@ -69,8 +76,8 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t w) {
     return w;
 }
 
-// Products of N fragments, each read from LDS DEPTH products before its own.  The order is kept as written
-// (by itself the compiler reads, waits, multiplies).
+// Products of N fragments, each read from LDS DEPTH products before its own.  The order is kept four products
+// by four (by itself the compiler reads, waits, multiplies; one by one is 2 to 5 % slower).
 template <int N, int DEPTH, typename Frag, typename Read, typename Product>
 __device__ __forceinline__ void products(Read read, Product product) {
     Frag f[DEPTH];
@@ -80,8 +87,17 @@ __device__ __forceinline__ void products(Read read, Product product) {
     for (int i = 0; i < N; ++i) {
         product(i, f[i % DEPTH]);
         if (i + DEPTH < N) f[i % DEPTH] = read(i + DEPTH);
-        __builtin_amdgcn_sched_barrier(0);
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
+}
+
+// The values of lanes r and r + 32, to both.
+__device__ __forceinline__ f32x2 both_halves(float x) {
+    // (of the builtin's two results this compiler uses the first one for both; the wait is for the registers'
+    // writes just before)
+    float lo = x, hi = x;
+    asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(lo), "+v"(hi));
+    return f32x2{lo, hi};
 }
 
 // A workgroup's place: PR_ROWS (token, head) pairs of sequence b, from its f0-th of nf on, of which the
@@ -191,10 +207,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
     constexpr int RI = 512 / D;            // tokens of one wave load
     constexpr int NL = 16 / RI;            // loads of a wave and tile, for K and for V
     constexpr int DEPTH = D == 64 ? 4 : 6; // fragments read ahead
+    constexpr int NP = NS * KS;            // products of a tile's scores; as many of its outputs
+    static_assert(NP == 4 * NL && NP == NS * D / 16, "a load every other product");
+    constexpr int KM = D == 64 ? 7 : 15, KQ = (KM + 1) / 2; // K's chunks: swizzle, offsets of a lane
     constexpr uint32_t ALL = (1u << NB) - 1;
     static_assert(NB == 4, "a block a wave");
-    __shared__ __attribute__((aligned(16))) T s_k[2][BN * D];
-    __shared__ __attribute__((aligned(16))) T s_v[2][BN * D];
+    // Two tiles, each an array of its own: the compiler has reads wait for loads to the same array.
+    __shared__ __attribute__((aligned(16))) T s_k0[BN * D], s_k1[BN * D], s_v0[BN * D], s_v1[BN * D];
     __shared__ int s_bad;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
@@ -249,23 +268,22 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
         if (t + 1 < nt) pg_next = look_up(t + 1);
     };
     // Every wave loads its block.  Tokens that are not there are taken from a place that is (masked below).
-    auto stage_load = [&](const uint8_t *base, T *lds, bool values) {
-#pragma unroll
-        for (int p = 0; p < NL; ++p) {
-            const int key = p * RI + lane / (D / 8), ch = lane % (D / 8); // of the block
-            const int t = max(0, min(key, toks - 1));
-            lds_load16(base + off, (uint32_t)(t * ts2 + (ch ^ (values ? 2 * (key & 3) : key & 7)) * 16),
-                       lds + (wave * NL + p) * 512);
-        }
+    // Load x of 2 NL: the keys', then the values'.
+    auto stage_load = [&](T *to_k, T *to_v, int x) {
+        const bool values = x >= NL;
+        const int p = x % NL, key = p * RI + lane / (D / 8), ch = lane % (D / 8); // of the block
+        const int t = max(0, min(key, toks - 1));
+        lds_load16((values ? vb : kb) + off, (uint32_t)(t * ts2 + (ch ^ (values ? 2 * (key & 3) : key & KM)) * 16),
+                   (values ? to_v : to_k) + (wave * NL + p) * 512);
     };
 
     f32x16 o[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) o[i] = f32x16{};
     float m = -INFINITY, l = 0.f; // the maximum that weights are taken against, and this lane's sum
-    uint32_t ko[4], vo[2];
+    uint32_t ko[KQ], vo[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ko[i] = r * (D * 2) + (((2 * i + h) ^ (r & 7)) * 16);
+    for (int i = 0; i < KQ; ++i) ko[i] = r * (D * 2) + (((2 * i + h) ^ (r & KM)) * 16);
     {
         const int j = (lane & 15) >> 2, c = 2 * (r >> 4) + ((lane & 3) >> 1); // token, chunk of its first 64 bytes
         vo[0] = (4 * h + j) * (D * 2) + ((c ^ (2 * j)) * 16) + 8 * (lane & 1);
@@ -274,8 +292,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
 
     if (first_t < nt) {
         stage(first_t);
-        stage_load(kb, s_k[first_t & 1], false);
-        stage_load(vb, s_v[first_t & 1], true);
+#pragma unroll
+        for (int x = 0; x < 2 * NL; ++x) stage_load(s_k0, s_v0, x);
     }
     x8 qf[KS];
     const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u; // a negative scale: -q, exactly
@@ -284,99 +302,106 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
     bool fresh = true, part = false;
     uint32_t ok = 0;
     int first_part = nt; // the first tile that some row does not see all of
-    for (int t = first_t; t < nt;) {
+    int t = first_t;
+    float mx;
+    // Works on tile t; true: it is done, and another one follows.
+    auto tile = [&](T *k_now, T *v_now, T *k_next, T *v_next) {
+        const uint8_t *lk = (const uint8_t *)k_now;
+        if (fresh) {
+            ok = okay;
+            part = (t + 1) * BN > pl.full || ok != ALL;
+            lds_loaded();
+            __syncthreads(); // tile t is there, and nobody works on tile t - 1
+            // A value that a row does not see meets a weight of 0, which an infinity or NaN would survive:
+            // in such a tile those are 0 for the products, and the rows that see them get them at the end.
+            if (part) {
+                first_part = min(first_part, t);
+                constexpr int NW = BN * D / 8 / 256;
+                u32x4 w[NW];
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < NW; ++i) w[i] = ((const u32x4 *)v_now)[tid + 256 * i];
+#pragma unroll
+                for (int i = 0; i < NW; ++i) {
+                    bool any = false;
+                    for (int j = 0; j < 4; ++j) any |= not_finite<T>(w[i][j]);
+                    if (any) {
+                        for (int j = 0; j < 4; ++j) w[i][j] = finite_only<T>(w[i][j]);
+                        ((u32x4 *)v_now)[tid + 256 * i] = w[i];
+                        bad = true;
+                    }
+                }
+                if (bad) s_bad = 1;
+                __syncthreads();
+            }
+        }
+        f32x16 s[NS];
+        auto read_k = [&](int x) { // the score tiles in turn: two chains of sums
+            const int i = x % NS, k = x / NS;
+            return *(const x8 *)(lk + ko[k % KQ] + i * (32 * D * 2) + (k / KQ) * (32 * KQ));
+        };
+        auto score = [&](int x, x8 kf) { s[x % NS] = E::mfma32(kf, qf[x / NS], x < NS ? f32x16{} : s[x % NS]); };
+        // The next tile's loads go out between the products: all at once would hold the wave up.
+        if (fresh && t + 1 < nt) {
+            stage(t + 1);
+            products<NP, DEPTH, x8>(read_k, [&](int x, x8 kf) {
+                score(x, kf);
+                if (x % 2 == 0) stage_load(k_next, v_next, x / 2);
+            });
+        } else products<NP, DEPTH, x8>(read_k, score);
+        if (part)
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int key = 32 * i + 8 * (j >> 2) + 4 * h + (j & 3);
+                    if (t * BN + key >= seen || !(ok >> (2 * i + (j >> 3)) & 1)) s[i][j] = -INFINITY;
+                }
+        mx = s[0][0];
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[i][j]);
+        const f32x2 mb = both_halves(mx);
+        mx = fmaxf(mb.x, mb.y) * scale;
+        if (t == first_t) m = fmaxf(m, mx); // nothing to rescale yet
+        fresh = !__any(mx > m + LAZY);
+        if (!fresh) return false;
+        const float base = base_of(m) - SHIFT<T>;
+        float sum = 0.f;
+        u32x4 pw[2 * NS]; // the weights, in P^T's operand layout
+        auto weights = [&](int k, int w) { // of block k's word w
+            const int i = k / 2, j = k % 2 * 8 + 2 * w;
+            const float p0 = exp2_(__builtin_fmaf(s[i][j], scale, -base));
+            const float p1 = exp2_(__builtin_fmaf(s[i][j + 1], scale, -base));
+            sum += p0 + p1;
+            pw[k][w] = E::pack(p0, p1);
+        };
+#pragma unroll
+        for (int w = 0; w < 4; ++w) weights(0, w);
+        const MOE_LDS uint8_t *const lv[2] = {lds_at(v_now, vo[0]), lds_at(v_now, vo[1])};
+        auto read_v = [&](int x) {
+            const int k = x / (D / 32), i = x % (D / 32);
+            const MOE_LDS uint8_t *p = lv[i & 1] + k * (16 * D * 2) + (i >> 1) * 128;
+            const u32x2 v0 = lds_read_tr(p), v1 = lds_read_tr(p + 8 * D * 2);
+            return __builtin_bit_cast(x8, (u32x4{v0.x, v0.y, v1.x, v1.y}));
+        };
+        products<NP, DEPTH, x8>(read_v, [&](int x, x8 vf) {
+            const int k = x / (D / 32), i = x % (D / 32);
+            o[i] = E::mfma32(vf, __builtin_bit_cast(x8, pw[k]), o[i]);
+            // the next block's weights, beside this one's products
+            for (int w = 4 * i / (D / 32); k + 1 < NB && w < 4 * (i + 1) / (D / 32); ++w) weights(k + 1, w);
+        });
+        l += sum;
+        return ++t < nt;
+    };
+    while (t < nt) {
         // Tiles until a row's maximum grows past what its weights allow for; then the outputs are rescaled
         // and the tile's scores computed again.  (Two loops, so that the inner one's outputs are the
         // products' own and stay where those put them.)
-        float mx;
         for (;;) {
-            const int buf = t & 1;
-            const uint8_t *lk = (const uint8_t *)s_k[buf], *lv = (const uint8_t *)s_v[buf];
-            if (fresh) {
-                ok = okay;
-                part = (t + 1) * BN > pl.full || ok != ALL;
-                lds_loaded();
-                __syncthreads(); // tile t is there, and nobody works on tile t - 1
-                // A value that a row does not see meets a weight of 0, which an infinity or NaN would survive:
-                // in such a tile those are 0 for the products, and the rows that see them get them at the end.
-                if (part) {
-                    first_part = min(first_part, t);
-                    constexpr int NW = BN * D / 8 / 256;
-                    u32x4 w[NW];
-                    bool bad = false;
-#pragma unroll
-                    for (int i = 0; i < NW; ++i) w[i] = ((const u32x4 *)s_v[buf])[tid + 256 * i];
-#pragma unroll
-                    for (int i = 0; i < NW; ++i) {
-                        bool any = false;
-                        for (int j = 0; j < 4; ++j) any |= not_finite<T>(w[i][j]);
-                        if (any) {
-                            for (int j = 0; j < 4; ++j) w[i][j] = finite_only<T>(w[i][j]);
-                            ((u32x4 *)s_v[buf])[tid + 256 * i] = w[i];
-                            bad = true;
-                        }
-                    }
-                    if (bad) s_bad = 1;
-                    __syncthreads();
-                }
-                if (t + 1 < nt) {
-                    stage(t + 1);
-                    stage_load(kb, s_k[buf ^ 1], false);
-                    stage_load(vb, s_v[buf ^ 1], true);
-                }
-            }
-            f32x16 s[NS];
-            products<NS * KS, DEPTH, x8>(
-                [&](int x) { // the score tiles in turn: two chains of sums
-                    const int i = x % NS, k = x / NS;
-                    return *(const x8 *)(lk + ko[k & 3] + i * (32 * D * 2) + (k >> 2) * 128);
-                },
-                [&](int x, x8 kf) {
-                    const int i = x % NS, k = x / NS;
-                    s[i] = E::mfma32(kf, qf[k], k ? s[i] : f32x16{});
-                });
-            if (part)
-#pragma unroll
-                for (int i = 0; i < NS; ++i)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int key = 32 * i + 8 * (j >> 2) + 4 * h + (j & 3);
-                        if (t * BN + key >= seen || !(ok >> (2 * i + (j >> 3)) & 1)) s[i][j] = -INFINITY;
-                    }
-            mx = s[0][0];
-#pragma unroll
-            for (int i = 0; i < NS; ++i)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[i][j]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32)) * scale;
-            if (t == first_t) m = fmaxf(m, mx); // nothing to rescale yet
-            fresh = !__any(mx > m + LAZY);
-            if (!fresh) break;
-            const float base = base_of(m) - SHIFT<T>;
-            float sum = 0.f;
-            u32x4 pw[2 * NS]; // the weights, in P^T's operand layout
-#pragma unroll
-            for (int i = 0; i < NS; ++i)
-#pragma unroll
-                for (int j = 0; j < 16; j += 2) {
-                    const float p0 = exp2_(__builtin_fmaf(s[i][j], scale, -base));
-                    const float p1 = exp2_(__builtin_fmaf(s[i][j + 1], scale, -base));
-                    sum += p0 + p1;
-                    pw[2 * i + (j >> 3)][(j & 7) >> 1] = E::pack(p0, p1);
-                }
-            l += sum;
-            products<NS * D / 16, DEPTH, x8>(
-                [&](int x) {
-                    const int k = x / (D / 32), i = x % (D / 32);
-                    const uint8_t *p = lv + vo[i & 1] + k * (16 * D * 2) + (i >> 1) * 128;
-                    const u32x2 v0 = lds_read_tr(p), v1 = lds_read_tr(p + 8 * D * 2);
-                    return __builtin_bit_cast(x8, (u32x4{v0.x, v0.y, v1.x, v1.y}));
-                },
-                [&](int x, x8 vf) {
-                    const int k = x / (D / 32), i = x % (D / 32);
-                    o[i] = E::mfma32(vf, __builtin_bit_cast(x8, pw[k]), o[i]);
-                });
-            if (++t == nt) break;
+            if (((t - first_t) & 1) == 0 && !tile(s_k0, s_v0, s_k1, s_v1)) break;
+            if (!tile(s_k1, s_v1, s_k0, s_v0)) break;
         }
         if (t < nt) {
             const float mn = fmaxf(m, mx);
@@ -411,7 +436,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
         }
 
     // ---- rows out, or their part
-    const float sum = l + __shfl_xor(l, 32);
+    const f32x2 lb = both_halves(l);
+    const float sum = lb.x + lb.y;
     if (!whole) {
         if (!valid) return;
         const size_t pr = part_row(pl, pl.piece) + wave * 32 + r;
@@ -427,8 +453,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
     // Through LDS, so that whole rows are stored: a wave's rows in a part of its own, 16 bytes between them.
     // (The tiles are done with: the barrier before the infinities.)
     constexpr int OS = D + 8;
-    static_assert(128 * OS <= 4 * BN * D, "the rows in the tiles' place");
-    T *so = (wave < 2 ? s_k[0] : s_v[0]) + (wave & 1) * 32 * OS;
+    static_assert(32 * OS <= BN * D, "the rows in the tiles' place");
+    T *so = (wave == 0 ? s_k0 : wave == 1 ? s_k1 : wave == 2 ? s_v0 : s_v1);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
