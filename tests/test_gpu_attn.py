@@ -897,3 +897,14 @@ def test_cut_prompts_of_odd_heads_in_a_padded_batch(gpu, heads):
 def test_prompt_around_the_length_that_is_cut(gpu, n):
     log(f"prompt of 3 rows, {n} cached")
     run_decode(gpu, Setup(8, 2, 64, 16, "bf16", [n, 100], [3, 60], seed=51))
+
+
+@pytest.mark.parametrize("heads", [(32, 8, 64), (16, 2, 256), (64, 16, 128)])
+def test_prompts_of_many_weights(gpu, heads):
+    """More tiles than are at work at once, of sequences of all lengths in no order, some with rows in front of
+    the cache: each tile is worked on, once."""
+    log(f"prompts of many weights {heads}")
+    rows = [(193 * b + 71) % 260 for b in range(24)]
+    before = [(389 * b) % 700 - 60 if b % 3 else 0 for b in range(24)]
+    kv = [max(0, r + c) for r, c in zip(rows, before)]
+    run_decode(gpu, Setup(*heads, 32, "bf16", kv, rows, seed=52, extra_rows=1))
