@@ -22,6 +22,10 @@
 //     is element 8 m + j, which only the output's addressing sees.
 //   * A wave's loads of the next 32 tokens' K are issued before the softmax, those of V after the
 //     products.
+// 64 sequences of 202 to 16384 tokens, 16/2 heads of 256: 90 us, 4.9 TB/s of K and V; one of 128k tokens 57 us,
+// 4.7 TB/s (this launch alone 5.3 TB/s; a kernel that only reads reaches 6.1).  256 sequences of 1 to 2048, 32/8 heads of
+// 128: 66 us, 4.1 TB/s.  One of 512 tokens: 11 us, two launches and the chain lengths -> pages -> K -> V.
+// The same kernel with one workgroup a unit and no cut: 128k tokens 102 ms, 64 sequences 12.6 ms.
 #include "attn_device.hpp"
 
 namespace moe {
@@ -297,9 +301,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
 // row through all of them.  More: a row at a time, a thread four elements of every PG-th piece, JOIN_B of
 // them under way.
 constexpr int JOIN_FEW = 16, JOIN_B = 16;
-template <typename T, int D, int THREADS>
+template <typename T, int D, int W, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_wg) {
-    constexpr int TPR = D / 4, PG = THREADS / TPR;
+    constexpr int TPR = W / 4, PG = THREADS / TPR; // W elements of a row, gridDim.z times
+    const int d0 = (int)blockIdx.z * W;
     __shared__ float s_f[DEC_MAX_WG];
     __shared__ f32x4 s_x[PG][TPR];
     const Piece pc = {ldc(&a.piece[blockIdx.x].b), ldc(&a.piece[blockIdx.x].hb), ldc(&a.piece[blockIdx.x].w0),
@@ -316,7 +321,7 @@ __global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_
     auto row = [&](int r, int p) { return slot(p) * DEC_HEADS + r; };
     if (n <= JOIN_FEW) {
         for (int i = r0 * TPR + tid; i < r1 * TPR; i += THREADS) {
-            const int r = i / TPR, d = i % TPR * 4;
+            const int r = i / TPR, d = d0 + i % TPR * 4;
             f32x2 ml[JOIN_FEW];
             f32x4 v[JOIN_FEW];
 #pragma unroll
@@ -338,7 +343,7 @@ __global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_
         }
         return;
     }
-    const int pg = tid / TPR, d = tid % TPR * 4;
+    const int pg = tid / TPR, d = d0 + tid % TPR * 4;
     for (int r = r0; r < r1; ++r) {
         f32x4 v[JOIN_B];
         auto load = [&](int p) {
@@ -379,14 +384,18 @@ __global__ __launch_bounds__(THREADS) void k_attn_join(AttnArgs a, int rows_per_
 template <typename T, int D>
 hipError_t decode_d(const AttnArgs &a, hipStream_t st) {
     k_attn_decode<T, D><<<a.n_wg, 256, 0, st>>>(a);
-    // Few units, so possibly many pieces each: one row a workgroup of 512.  Many, so a few pieces of each
-    // mostly: the rows that 256 threads hold.
+    // Few units, so possibly many pieces each: one row a workgroup, or 64 elements of it where the page lists
+    // hold more than 64 steps.  (One sequence of 128k tokens, 16/2 heads of 256: 58.8 us by rows, 56.7 by 64
+    // elements with the decode; of 512 tokens 10.7 and 10.9; 256 sequences, as many slices as 4096, 66 and 69.)
+    // Many units, so a few pieces of each mostly: the rows that 256 threads hold.
     const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS, rows = a.group < DEC_HEADS ? a.group : DEC_HEADS;
     const int64_t units = (int64_t)a.n_seqs * a.hkv * gb;
     const int x = units <= a.n_wg ? (int)units : a.n_wg, per = 1024 / D;
-    if (x * rows <= 512) k_attn_join<T, D, 512><<<dim3(x, rows), 512, 0, st>>>(a, 1);
-    else if (x * rows <= 2048) k_attn_join<T, D, 256><<<dim3(x, rows), 256, 0, st>>>(a, 1);
-    else k_attn_join<T, D, 256><<<dim3(x, (rows + per - 1) / per), 256, 0, st>>>(a, per);
+    const bool longer = (int64_t)a.max_pages << a.page_shift > 64 * DEC_STEP;
+    if (longer && x * rows * (D / 64) <= 256) k_attn_join<T, D, 64, 256><<<dim3(x, rows, D / 64), 256, 0, st>>>(a, 1);
+    else if (x * rows <= 512) k_attn_join<T, D, D, 512><<<dim3(x, rows), 512, 0, st>>>(a, 1);
+    else if (x * rows <= 2048) k_attn_join<T, D, D, 256><<<dim3(x, rows), 256, 0, st>>>(a, 1);
+    else k_attn_join<T, D, D, 256><<<dim3(x, (rows + per - 1) / per), 256, 0, st>>>(a, per);
     return hipGetLastError();
 }
 

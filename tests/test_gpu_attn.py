@@ -908,3 +908,10 @@ def test_prompts_of_many_weights(gpu, heads):
     before = [(389 * b) % 700 - 60 if b % 3 else 0 for b in range(24)]
     kv = [max(0, r + c) for r, c in zip(rows, before)]
     run_decode(gpu, Setup(*heads, 32, "bf16", kv, rows, seed=52, extra_rows=1))
+
+
+@pytest.mark.parametrize("heads", [(4, 2, 64), (6, 1, 128), (16, 1, 256), (20, 1, 256)])
+@pytest.mark.parametrize("kv", [[8192], [8193, 0], [8300, 17, 4000]])
+def test_decode_around_64_steps(gpu, heads, kv):
+    log(f"decode {heads} over {kv}")
+    run_decode(gpu, Setup(*heads, 16, "bf16", kv, seed=53, pad_pages=0))
