@@ -287,7 +287,7 @@ typedef struct {
 /* A cache: element (page, head, token, i) of the keys at
  *   k + page * page_stride + head * head_stride + token * token_stride + i   (elements),
  * the values with the same strides from v.  Any order of page, head and token; strides are
- * multiples of 8 elements and head_dim at least, token_stride 2^24 at most, k and v 16-byte
+ * multiples of 8 elements and head_dim at least, token_stride 2^22 at most, k and v 16-byte
  * aligned, i contiguous. */
 typedef struct {
     void *k, *v;

@@ -70,8 +70,8 @@ moe_status common_args(const char *fn, moe_attn *a, const moe_kv_cache *kv, cons
     if (kv->n_pages < 1) return fail(MOE_EINVAL, "%s: a cache of %d pages", fn, kv->n_pages);
     const int64_t strides[3] = {kv->page_stride, kv->head_stride, kv->token_stride};
     for (int64_t v : strides)
-        if (v < g.head_dim || (v & 7) || v > ((int64_t)1 << 40) || kv->token_stride > (1 << 24))
-            return fail(MOE_EINVAL, "%s: cache stride %lld (multiples of 8, head_dim=%d at least; token_stride at most 2^24)", fn,
+        if (v < g.head_dim || (v & 7) || v > ((int64_t)1 << 40) || kv->token_stride > (1 << 22)) // (bytes in 24 bits)
+            return fail(MOE_EINVAL, "%s: cache stride %lld (multiples of 8, head_dim=%d at least; token_stride at most 2^22)", fn,
                         (long long)v, g.head_dim);
     if (kv->n_pages > ((int64_t)1 << 46) / kv->page_stride)
         return fail(MOE_EINVAL, "%s: %d pages %lld elements apart", fn, kv->n_pages, (long long)kv->page_stride);

@@ -267,7 +267,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
     // ---- tiles
     const int32_t *pages = a.pages + pl.b * a.pages_stride;
     const uint8_t *kb = a.k + 2 * pl.hk * a.head_stride, *vb = a.v + 2 * pl.hk * a.head_stride;
-    const int ts2 = (int)(2 * a.token_stride), mask = (1 << a.page_shift) - 1;
+    const uint32_t ts2 = (uint32_t)(2 * a.token_stride); // (below 2^24)
+    const int mask = (1 << a.page_shift) - 1;
     // Lane i has the page of block i of the tile to be staged next (-1: none); okay: the blocks of the tile
     // staged last that have a page of the cache, or no token to be seen.
     bool bad_page = false;
@@ -300,7 +301,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
         const bool values = x >= NL;
         const int p = x % NL, key = p * RI + lane / (D / 8), ch = lane % (D / 8); // of the block
         const int t = max(0, min(key, toks - 1));
-        lds_load16((values ? vb : kb) + off, (uint32_t)(t * ts2 + (ch ^ (values ? 2 * (key & 3) : key & KM)) * 16),
+        lds_load16((values ? vb : kb) + off, __umul24(t, ts2) + (ch ^ (values ? 2 * (key & 3) : key & KM)) * 16,
                    (values ? to_v : to_k) + (wave * NL + p) * 512);
     };
 

@@ -915,3 +915,30 @@ def test_prompts_of_many_weights(gpu, heads):
 def test_decode_around_64_steps(gpu, heads, kv):
     log(f"decode {heads} over {kv}")
     run_decode(gpu, Setup(*heads, 16, "bf16", kv, seed=53, pad_pages=0))
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 2.0])
+@pytest.mark.parametrize("heads, rows", [((8, 2, 64), [3, 50]), ((16, 2, 256), [20, 1]), ((8, 2, 128), None)])
+def test_scales_of_pieces(gpu, scale, heads, rows):
+    log(f"scale {scale} of pieces, {heads} rows {rows}")
+    run_decode(gpu, Setup(*heads, 16, "f16", [3500, 900], rows, seed=54), scale=scale)
+
+
+@pytest.mark.parametrize("rows", [None, [30, 5]])
+def test_tokens_far_apart(gpu, rows):
+    """The largest token stride: a page's tokens 8 MiB apart (and 256 MiB from its first to its last)."""
+    import torch
+    log(f"token stride 2^22, rows {rows}")
+    s = Setup(2, 1, 64, 32, "f16", [35, 5], rows, seed=55)
+    small = s.pools()
+    stride = 1 << 22
+    buf = torch.empty(2, 32 * stride, dtype=torch.float16, device="cuda")
+    far = [torch.as_strided(buf[i], (s.n_pages, 1, 32, 64), (64, 64 * s.n_pages, stride, 1)) for i in range(2)]
+    for f, x in zip(far, small):
+        f.copy_(x)
+    far = [torch.as_strided(f, f.shape, (64, 64, stride, 1), f.storage_offset()) for f in far]
+    want, bound, _, _ = s.reference()
+    ctx = s.context(gpu)
+    call = ctx.attn_decode if rows is None else ctx.attn_prompt
+    check("o", call(gpu.KVCache(*far), s.seqs(gpu), s.q.cuda()), want, bound)
+    assert ctx.device_flags() == 0
