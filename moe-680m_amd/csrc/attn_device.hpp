@@ -88,6 +88,62 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
     return x;
 }
 
+// 2^shift sets of 64 sequences make a group, of which there are up to 64.
+__device__ __forceinline__ int group_shift(int n_seqs) {
+    int shift = 0;
+    while ((n_seqs - 1) >> (12 + shift)) ++shift;
+    return shift;
+}
+// Something counted for each sequence (count(b) for any b, 0 behind the last one): of up to 64 sequences lane b has
+// sequence b's, of more lane c those of the c-th of up to 64 groups; incl: with all in front.  All four waves
+// of a workgroup call it, and share the sequences where they are many.  Neighbours' loads lie side by side
+// (each lane of every wave a run of sequences, the run searched one by one: 4096 prompts of 16 rows 541 us, so
+// 142; 1024 of them 42, 25).
+template <typename Count>
+__device__ __forceinline__ void count_seqs(int n_seqs, int lane, int wave, Count count, uint32_t &mine, uint32_t &incl) {
+    if (n_seqs <= 64) mine = count(lane);
+    else {
+        constexpr int AT_ONCE = 4;
+        __shared__ uint32_t s_mine[4][64];
+        const int sets = (n_seqs + 63) / 64, shift = group_shift(n_seqs);
+        mine = 0;
+        for (int k = wave * AT_ONCE; k < sets; k += 4 * AT_ONCE) {
+            uint32_t n[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) n[i] = count((k + i) * 64 + lane);
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const uint32_t sum = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(n[i]), 63);
+                mine += lane == (k + i) >> shift ? sum : 0u;
+            }
+        }
+        s_mine[wave][lane] = mine;
+        __syncthreads();
+        mine = (s_mine[0][lane] + s_mine[1][lane]) + (s_mine[2][lane] + s_mine[3][lane]);
+    }
+    incl = wave_scan(mine);
+}
+// The sequence that has the want-th of what was counted, and what is in front of it; `from`: the lane that
+// counted it last.
+template <typename Count>
+__device__ __forceinline__ int find_seq(int n_seqs, int lane, Count count, uint32_t mine, uint32_t incl, uint32_t want,
+                                        uint32_t &before, int &from) {
+    from = __builtin_ctzll(__ballot(incl > want));
+    before = (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), from);
+    if (n_seqs <= 64) return from;
+    const int shift = group_shift(n_seqs), last = ((from + 1) << shift) - 1;
+    for (int k = from << shift;; ++k) {
+        const uint32_t n = count(k * 64 + lane), upto = before + wave_scan(n);
+        const uint64_t in = __ballot(upto > want);
+        if (in || k >= last) { // (none: the counts changed during the call)
+            from = in ? __builtin_ctzll(in) : 0;
+            before = (uint32_t)__builtin_amdgcn_readlane((int)(upto - n), from);
+            return min(k * 64 + from, n_seqs - 1);
+        }
+        before = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    }
+}
+
 // The largest of the wave's lanes.
 __device__ __forceinline__ uint32_t wave_most(uint32_t x) {
     x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, false)); // as above

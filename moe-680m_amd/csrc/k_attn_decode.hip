@@ -35,8 +35,8 @@ namespace {
 constexpr int DEC_STEP = DEC_WAVES * DEC_WAVE_TOK;
 
 // Steps of a sequence's units: one at least, so that an empty one's rows are written too.
-__device__ __forceinline__ int seq_steps(const AttnArgs &a, int b, int cap) {
-    return max(1, (min(max(a.kv_len[b], 0), cap) + DEC_STEP - 1) / DEC_STEP);
+__device__ __forceinline__ int steps(int len, int cap) {
+    return max(1, (min(max(len, 0), cap) + DEC_STEP - 1) / DEC_STEP);
 }
 
 // A partial row's maximum and sum: those of a row place lie together, so that a wave loads many
@@ -64,15 +64,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
     const int gb = (a.group + DEC_HEADS - 1) / DEC_HEADS; // head blocks of a key-value head
     const int ng = a.hkv * gb;                            // units of a sequence
 
-    // ---- this workgroup's run of steps [lo, hi): every wave sums the sequences' steps by itself,
-    // a lane those of `per` in a row, and finds the sequence that lo lies in
-    const int per = (a.n_seqs + 63) / 64;
-    uint32_t mine = 0;
-    for (int i = 0; i < per; ++i) {
-        const int b = lane * per + i;
-        if (b < a.n_seqs) mine += (uint32_t)seq_steps(a, b, cap);
-    }
-    const uint32_t incl = wave_scan(mine);
+    // ---- this workgroup's run of steps [lo, hi): every wave has the sequences' steps and finds the sequence
+    // that lo lies in
+    auto steps_of = [&](int b) {
+        const int n = steps(ldg<int>(a.kv_len + min(b, a.n_seqs - 1)), cap);
+        return b < a.n_seqs ? (uint32_t)n : 0u;
+    };
+    uint32_t mine, incl;
+    count_seqs(a.n_seqs, lane, wave, steps_of, mine, incl);
     const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63) * ng;
     const uint32_t share = (total + gridDim.x - 1) / gridDim.x;
     const uint32_t lo = blockIdx.x * share;
@@ -85,13 +84,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
         return;
     }
     const uint32_t hi = min(lo + share, total);
-    const int owner = __builtin_ctzll(__ballot(incl * ng > lo));
-    uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), owner); // steps before b, of one unit each
-    int b = owner * per, nt = uniform(seq_steps(a, b, cap));
-    while ((at + nt) * ng <= lo && b + 1 < a.n_seqs) {
-        at += nt;
-        nt = uniform(seq_steps(a, ++b, cap));
-    }
+    uint32_t at; // steps before b, of one unit each
+    int from, b = find_seq(a.n_seqs, lane, steps_of, mine, incl, lo / ng, at, from);
+    int nt = steps(ldc(a.kv_len + b), cap);
     // (a head block or sequence out of range, here and below: the lengths changed during the call)
     int hb = min((int)((lo - at * ng) / (uint32_t)nt), ng - 1);
     uint32_t unit = at * ng + hb * nt; // first step of unit (b, hb)
@@ -289,7 +284,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_decode(AttnArgs a) {
         if (++hb == ng) {
             hb = 0;
             if (++b >= a.n_seqs) break;
-            nt = uniform(seq_steps(a, b, cap));
+            nt = steps(ldc(a.kv_len + b), cap);
         }
     }
     if (bad && lane == 0) raise(a.flags, MOE_DEVFLAG_BAD_PAGE);

@@ -117,28 +117,28 @@ struct Place {
 // tokens lie on one XCD (workgroups go round the XCDs in turn), side by side.  (No loop runs on and no
 // index leaves its array if the lengths and rows should change under the call.)
 template <int D, bool JOIN>
-__device__ __forceinline__ bool find_place(const AttnArgs &a, int lane, bool flag, Place &pl) {
+__device__ __forceinline__ bool find_place(const AttnArgs &a, int lane, int wave, bool flag, Place &pl) {
     const int cap = a.max_pages << a.page_shift;
-    const int per = (a.n_seqs + 63) / 64;
-    auto tiles = [&](int n) { return ((uint32_t)n * a.group + PR_ROWS - 1) / PR_ROWS; };
-    uint32_t mine = 0;
+    uint32_t mine, incl;
     int most = 0; // tokens that a row sees
     bool bad = false;
-    Rows sr = {};
-    for (int i = 0; i < per; ++i) {
-        const int b = lane * per + i;
-        if (b < a.n_seqs) {
-            sr = seq_rows(a, b);
-            bad |= sr.bad;
-            mine += tiles(sr.n);
-            if (sr.n > 0) {
-                bad |= sr.len < 0 || sr.len > cap;
-                most = max(most, min(sr.len, cap));
-            }
-        }
-    }
+    Rows sr = {}; // of the sequence that the lane looked at last
+    auto tiles_of = [&](int b) {
+        sr = seq_rows(a, min(b, a.n_seqs - 1));
+        if (b >= a.n_seqs) sr.n = 0;
+        bad |= sr.bad || (sr.n > 0 && (sr.len < 0 || sr.len > cap));
+        most = max(most, sr.n > 0 ? min(sr.len, cap) : 0);
+        return ((uint32_t)sr.n * a.group + PR_ROWS - 1) / PR_ROWS;
+    };
+    count_seqs(a.n_seqs, lane, wave, tiles_of, mine, incl);
     if (flag && bad) raise(a.flags, MOE_DEVFLAG_BAD_SEQ);
-    const uint32_t incl = wave_scan(mine);
+    if (a.n_seqs > 64 && a.splits > 1) { // each wave has looked at some
+        __shared__ int s_most[4];
+        most = (int)wave_most((uint32_t)most);
+        if (lane == 0) s_most[wave] = most;
+        __syncthreads();
+        most = max(max(s_most[0], s_most[1]), max(s_most[2], s_most[3]));
+    }
     const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
     if (total == 0) return false;
     uint32_t nth = blockIdx.x / a.hkv; // tile number, from the end
@@ -169,7 +169,7 @@ __device__ __forceinline__ bool find_place(const AttnArgs &a, int lane, bool fla
         nth = total - 1 - (nth - first);
     int from; // the lane that has the sequence
     uint32_t before; // the sequence's tiles before this one
-    if (per == 1 && a.n_seqs > 1 && pl.n == 1 && total > first) {
+    if (a.n_seqs <= 64 && a.n_seqs > 1 && pl.n == 1 && total > first) {
         // Tile j of a sequence, from its end, weighs `top` - j (in tiles of seen tokens).  The nth heaviest
         // one: of weight w, the largest one that more than nth reach, and among those of the same weight by
         // sequence.
@@ -192,17 +192,8 @@ __device__ __forceinline__ bool find_place(const AttnArgs &a, int lane, bool fla
         before = (uint32_t)__builtin_amdgcn_readlane((int)(mine - 1 - (uint32_t)(top - w)), from);
     } else {
         const uint32_t want = total - 1 - nth;
-        from = __builtin_ctzll(__ballot(incl > want));
-        uint32_t at = (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), from);
-        pl.b = from * per; // (one sequence a lane: this one has it)
-        if (per > 1)
-            for (from = 0;; ++pl.b) {
-                sr = seq_rows(a, pl.b);
-                const uint32_t n = uniform(tiles(sr.n));
-                if (want < at + n || pl.b + 1 >= a.n_seqs) break;
-                at += n;
-            }
-        before = want - at;
+        pl.b = find_seq(a.n_seqs, lane, tiles_of, mine, incl, want, before, from);
+        before = want - before;
     }
     auto of = [&](int v) { return __builtin_amdgcn_readlane(v, from); };
     pl.r0 = of(sr.r0);
@@ -246,7 +237,7 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void k_attn_prompt(AttnArgs 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int r = lane & 31, h = lane >> 5;
     Place pl;
-    if (!find_place<D, false>(a, lane, blockIdx.x == 0 && wave == 0, pl)) return;
+    if (!find_place<D, false>(a, lane, wave, blockIdx.x == 0, pl)) return;
     // this piece's tiles [t, nt); the first one also where no token is seen, to write the rows
     const int tiles = (pl.ext + BN - 1) / BN, first_t = pl.piece * pl.chunk;
     if (pl.piece > 0 && first_t >= tiles) return;
@@ -523,7 +514,7 @@ __global__ __launch_bounds__(256) void k_attn_prompt_join(AttnArgs a) {
     __shared__ f32x2 s_ml[PG];
     const int tid = threadIdx.x, i = tid % TPR, g = tid / TPR;
     Place pl;
-    if (!find_place<D, true>(a, tid & 63, false, pl)) return;
+    if (!find_place<D, true>(a, tid & 63, uniform(tid >> 6), false, pl)) return;
     const int tiles = (pl.ext + BN - 1) / BN, n = min(pl.n, (tiles + pl.chunk - 1) / pl.chunk);
     if (n < 2) return;
     const bool one = gridDim.y == PR_ROWS;

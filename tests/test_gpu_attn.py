@@ -942,3 +942,25 @@ def test_tokens_far_apart(gpu, rows):
     call = ctx.attn_decode if rows is None else ctx.attn_prompt
     check("o", call(gpu.KVCache(*far), s.seqs(gpu), s.q.cuda()), want, bound)
     assert ctx.device_flags() == 0
+
+
+@pytest.mark.parametrize("n", [64, 65, 700, 4096, 4097, 9000])
+def test_counts_of_many_sequences(gpu, n):
+    """Of a token or none each, and as many rows: every sequence's rows are found (one token: o is its value)."""
+    import torch
+    log(f"{n} sequences")
+    ctx = gpu.AttnContext(4, 2, 64, 16, n)
+    v = torch.randn((50, 2, 16, 64), device="cuda").half()
+    b = torch.arange(n, device="cuda", dtype=torch.int32)
+    pages = (b * 7 % 50).view(n, 1)
+    kv_len = ((b * 5 + b // 64) % 3 > 0).int()
+    cache = gpu.KVCache(torch.randn_like(v), v)
+    want = (v[pages[:, 0].long(), :, 0] * kv_len.view(n, 1, 1)).repeat_interleave(2, 1)
+    q = torch.randn((n, 4, 64), device="cuda").half()
+    assert torch.equal(ctx.attn_decode(cache, gpu.SeqBatch(pages, kv_len), q), want)
+    start = torch.zeros(n + 1, device="cuda", dtype=torch.int32)
+    start[1:] = kv_len.cumsum(0)
+    rows = int(start[-1])
+    o = ctx.attn_prompt(cache, gpu.SeqBatch(pages, kv_len, start, rows), q[:rows])
+    assert torch.equal(o, want[kv_len.bool()])
+    assert ctx.device_flags() == 0
